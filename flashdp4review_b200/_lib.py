@@ -9,7 +9,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 # FDP_B200_LIB points at another build of the same ABI (used to compare builds on one GPU)
 LIB_PATH = os.environ.get("FDP_B200_LIB") or os.path.join(PKG, "libfdp_b200.so")
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 FDP_OK = 0
 FDP_ERR_ARG, FDP_ERR_DTYPE, FDP_ERR_SHAPE, FDP_ERR_ALIGN = -1, -2, -3, -4
 FDP_ERR_WORKSPACE, FDP_ERR_ARCH, FDP_ERR_LAUNCH, FDP_ERR_TIMEOUT = -5, -6, -7, -8
@@ -20,6 +20,7 @@ FDP_OUT_IN, FDP_IN_OUT = 0, 1
 FDP_NORM_AUTO, FDP_NORM_DIRECT, FDP_NORM_GRAM = 0, 1, 2
 FDP_FP32_TENSOR, FDP_FP32_WIDE, FDP_KEEP_PRODUCTS, FDP_FP32_WIDE_GEMM, FDP_GEMM_SPLIT_K = 16, 32, 64, 128, 256
 FDP_PAD_16BIT = 512
+FDP_ACT_NONE, FDP_ACT_RELU, FDP_ACT_SILU, FDP_ACT_GELU, FDP_ACT_GELU_TANH = 0, 1, 2, 3, 4
 
 c_void_p, c_int, c_size_t, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 
@@ -31,6 +32,12 @@ class DPParams(ctypes.Structure):
                 ("param_id", ctypes.c_uint32), ("param_id2", ctypes.c_uint32),
                 ("step", ctypes.c_uint32), ("noise_rank", ctypes.c_int32),
                 ("noise_world", ctypes.c_int32), ("step_device", c_void_p)]
+
+
+class DropoutParams(ctypes.Structure):
+    """struct fdp_dropout_params"""
+    _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64),
+                ("stream_id", ctypes.c_uint32), ("step", ctypes.c_uint32), ("step_device", c_void_p)]
 
 
 # name -> (restype, argtypes); every function include/fdp_b200.h declares
@@ -68,6 +75,13 @@ SIGNATURES = {
     "fdp_layernorm_bwd_saturate": (c_int, [c_void_p] * 6 + [c_int] * 4 + [c_float, c_float, c_void_p, c_size_t, c_void_p]),
     "fdp_layernorm_bwd": (c_int, [c_void_p] * 10 + [c_int] * 5 +
                           [ctypes.POINTER(DPParams), c_void_p, c_size_t, c_void_p]),
+    "fdp_dropout": (c_int, [c_void_p, c_void_p, c_void_p, c_size_t, c_int, ctypes.POINTER(DropoutParams), c_void_p]),
+    "fdp_group_norm_fwd_workspace_bytes": (c_size_t, [c_int] * 4),
+    "fdp_group_norm_fwd": (c_int, [c_void_p] * 6 + [c_int] * 4 + [c_float] + [c_int] * 3 +
+                           [ctypes.POINTER(DropoutParams), c_void_p, c_size_t, c_void_p]),
+    "fdp_group_norm_bwd_workspace_bytes": (c_size_t, [c_int] * 4),
+    "fdp_group_norm_bwd": (c_int, [c_void_p] * 11 + [c_int] * 7 + [ctypes.POINTER(DropoutParams), ctypes.POINTER(DPParams),
+                                                                  c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

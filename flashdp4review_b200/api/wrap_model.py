@@ -15,12 +15,17 @@ import torch.nn as nn
 
 from ..layers.linear import DPLinear
 from ..layers.layernorm import DPLayerNorm
+from ..layers.groupnorm import DPGroupNorm
+from ..layers.dropout import DPDropout
 from ..layers.transformers_conv1d import DPConv1D, Conv1D
 
 dp_supported_modules = {
     nn.Linear: DPLinear,
     nn.LayerNorm: DPLayerNorm,
     Conv1D: DPConv1D,
+    # beyond the reference: the norm that networks over images use under DP-SGD, and dropout without a stored mask
+    nn.GroupNorm: DPGroupNorm,
+    nn.Dropout: DPDropout,
 }
 
 
@@ -43,6 +48,10 @@ def _twin_kwargs(module):
     if isinstance(module, nn.LayerNorm):
         return dict(normalized_shape=module.normalized_shape, eps=module.eps,
                     elementwise_affine=module.elementwise_affine)
+    if isinstance(module, nn.GroupNorm):
+        return dict(num_groups=module.num_groups, num_channels=module.num_channels, eps=module.eps, affine=module.affine)
+    if isinstance(module, nn.Dropout):
+        return dict(p=module.p, inplace=module.inplace)
     if isinstance(module, Conv1D):
         return dict(nf=module.nf, nx=module.weight.shape[0])
     raise NotImplementedError(f"Unsupported module type: {type(module)}")
@@ -51,8 +60,8 @@ def _twin_kwargs(module):
 def _replace(parent, prefix, chosen, kinds, hyper):
     for name, child in list(parent.named_children()):
         path = f"{prefix}.{name}" if prefix else name
-        if path in chosen and isinstance(child, kinds) and not getattr(child, "dp", False):
-            twin = _twin_class(child)(**_twin_kwargs(child), **hyper)
+        if path in chosen and isinstance(child, kinds) and not getattr(child, "dp", False) and not isinstance(child, DPDropout):
+            twin = _twin_class(child)(**_twin_kwargs(child), **(hyper if not isinstance(child, nn.Dropout) else {}))
             first = next(child.parameters(), None)
             if first is not None:
                 twin = twin.to(device=first.device, dtype=first.dtype)
@@ -67,8 +76,9 @@ def wrap_with_flashdp_layers(model, target_modules: List[Type[nn.Module]] = None
                              target_layers: List[str] = None, skip_layers: List[str] = None,
                              priority_to_target: bool = False, feedback: bool = True, C=1.0,
                              noise_multiplier=1.0, clamp_value=1.0) -> nn.Module:
-    """Replace the selected nn.Linear / nn.LayerNorm / transformers Conv1D layers of `model` by
-    DPLinear / DPLayerNorm / DPConv1D carrying (C, noise_multiplier, clamp_value); returns `model`.
+    """Replace the selected nn.Linear / nn.LayerNorm / nn.GroupNorm / transformers Conv1D layers of `model` by
+    DPLinear / DPLayerNorm / DPGroupNorm / DPConv1D carrying (C, noise_multiplier, clamp_value), and nn.Dropout by
+    DPDropout; returns `model`.
 
     Clip rule of every wrapped parameter tensor: g_b * min(C / (||g_b|| + 1e-10), clamp_value),
     averaged over the batch, plus N(0, (noise_multiplier/sqrt(B))^2).

@@ -3,5 +3,6 @@ from .ops import (  # noqa: F401
     layernorm_fwd_fused, layernorm_dw_clip, layernorm_db_clip, layernorm_bwd_clip_fused, layernorm_dwdb_fused,
     mm_fused,
     dp_linear_weight_grad, dp_bias_grad, dp_layernorm_backward, linear_input_grad, linear_forward,
+    DropoutSpec, dropout, dropout_backward, group_norm_forward, dp_group_norm_backward,
     RuntimeAutoTuner, NoiseSpec, noise_std,
 )

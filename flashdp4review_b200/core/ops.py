@@ -423,6 +423,119 @@ def layernorm_dwdb_fused(weight, bias, _dw, _db, args=None):
     return _dw.sum(0).to(weight.dtype), _db.sum(0).to(weight.dtype)
 
 
+# ------------------------------------------------------------------------------------------------
+# dropout
+# ------------------------------------------------------------------------------------------------
+@dataclass
+class DropoutSpec:
+    """Which mask one dropout call draws: a function of (p, seed, stream_id, step, offset, element index) alone, so nothing is
+    stored for the backward but this.  An element is dropped with probability p (to 2^-33) and the others are multiplied
+    by 1 / (1 - p).  `offset` counts groups of eight elements: ranks that draw for shards of one batch start apart."""
+    p: float = 0.5
+    seed: int = 0
+    stream_id: int = 0
+    step: int = 0
+    offset: int = 0
+    step_device: object = None    # a one-element int32 CUDA tensor the kernels add to `step` when they run
+
+
+def _drop(spec):
+    if spec is None:
+        return None
+    if not 0.0 <= spec.p <= 1.0:
+        raise ValueError(f"dropout probability has to be between 0 and 1, but got {spec.p}")
+    if not 0 <= spec.offset < 1 << 60:
+        raise ValueError(f"dropout offset has to be between 0 and 2^60, but got {spec.offset}")
+    return (float(spec.p), int(spec.seed) & (2 ** 64 - 1), int(spec.offset), int(spec.stream_id) & 0xFFFFFFFF,
+            int(spec.step) & 0xFFFFFFFF, spec.step_device.data_ptr() if spec.step_device is not None else None)
+
+
+def dropout(input, spec, residual=None, out=None):
+    """Dropout of `input` (plus `residual`, of the input's shape and dtype) under the mask of `spec`, elements numbered in
+    row-major order.  A dropped element is 0 whatever it held.  `out`: a contiguous tensor to write into; it may be the
+    input or the residual."""
+    host = _lib.host()
+    _require_cuda(input, residual, out)
+    code, d = _dt(input.dtype), _drop(spec)
+    if residual is not None and (residual.shape != input.shape or residual.dtype != input.dtype):
+        raise RuntimeError(f"residual must be a {tuple(input.shape)} tensor of {input.dtype}, "
+                           f"got {tuple(residual.shape)} of {residual.dtype}")
+    if out is not None and (out.shape != input.shape or out.dtype != input.dtype or out.device != input.device or not out.is_contiguous()):
+        raise RuntimeError(f"out must be a contiguous {tuple(input.shape)} tensor of {input.dtype} on {input.device}")
+    st, y = host.dropout(input.contiguous(), None if residual is None else residual.contiguous(), out, code, d)
+    _lib.check(st, "fdp_dropout")
+    return y
+
+
+def dropout_backward(grad_output, spec):
+    """The input's gradient of `dropout` with the same spec (the residual's is grad_output itself)."""
+    return dropout(grad_output, spec)
+
+
+# ------------------------------------------------------------------------------------------------
+# group norm, channels last
+# ------------------------------------------------------------------------------------------------
+ACTIVATIONS = {None: _lib.FDP_ACT_NONE, "relu": _lib.FDP_ACT_RELU, "silu": _lib.FDP_ACT_SILU, "gelu": _lib.FDP_ACT_GELU,
+               "gelu_tanh": _lib.FDP_ACT_GELU_TANH}
+
+
+def _activation(name):
+    try:
+        return ACTIVATIONS[name]
+    except KeyError:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {name!r}") from None
+
+
+def _group_norm_args(x, weight, bias, num_groups):
+    """(T, contiguous weight, contiguous bias, parameter dtype code) of a group norm over x (B, ..., C)"""
+    if x.dim() < 2:
+        raise RuntimeError(f"group norm needs an input (B, ..., C), got {tuple(x.shape)}")
+    C = x.shape[-1]
+    if num_groups < 1 or C % num_groups != 0:
+        raise ValueError(f"number of channels ({C}) must be divisible by num_groups ({num_groups})")
+    if (weight is None) != (bias is None):
+        raise ValueError("group norm has both a weight and a bias or neither")
+    if x.numel() == 0:
+        raise RuntimeError(f"group norm of an empty input {tuple(x.shape)}")
+    w = None if weight is None else weight.contiguous()
+    b = None if bias is None else bias.to(w.dtype).contiguous()
+    return x.numel() // (x.shape[0] * C), w, b, _lib.FDP_F32 if w is None else _dt(w.dtype)
+
+
+def group_norm_forward(input, weight, bias, num_groups, eps=1e-5, *, activation=None, dropout=None):
+    """dropout(activation(group_norm(input))) over channels-last input (B, ..., C), rounded once; returns (y,
+    {'mean', 'rstd'}) with fp32 statistics (B, num_groups).  weight / bias may be None.  `activation`: None, "relu",
+    "silu", "gelu" or "gelu_tanh"; `dropout`: a DropoutSpec, whose mask is that of `dropout(y, spec)`."""
+    host = _lib.host()
+    _require_cuda(input, weight, bias)
+    act, spec, code = _activation(activation), _drop(dropout), _dt(input.dtype)
+    x = input.contiguous()
+    T, w, b, pdt = _group_norm_args(x, weight, bias, num_groups)
+    st, y, mean, rstd = host.group_norm_fwd(x, w, b, T, num_groups, float(eps), act, code, pdt, spec)
+    _lib.check(st, "fdp_group_norm_fwd")
+    return y, {"mean": mean, "rstd": rstd}
+
+
+def dp_group_norm_backward(grad_output, input, weight, bias, mean, rstd, num_groups, C, clamp_value, *, activation=None,
+                           dropout=None, batch_divisor=None, noise=None, need_dx=True, need_dw=True, return_norms=False):
+    """(dx, dgamma, dbeta) of `group_norm_forward` with the same activation and dropout: dx as autograd's, dgamma and dbeta
+    from per-sample gradients that are each clipped by their norm, averaged and noised, as `dp_layernorm_backward`'s.  None
+    in the place of what is not needed; with return_norms the per-sample norms of both follow."""
+    host = _lib.host()
+    _require_cuda(grad_output, input, weight, bias, mean, rstd)
+    act, spec, code = _activation(activation), _drop(dropout), _dt(input.dtype)
+    x, dy = input.contiguous(), grad_output.to(input.dtype).contiguous()
+    T, w, b, pdt = _group_norm_args(x, weight, bias, num_groups)
+    need_dw = need_dw and w is not None
+    if not (need_dx or need_dw):
+        return (None,) * (5 if return_norms else 3)
+    st, dx, dgamma, dbeta, ng, nb = host.group_norm_bwd(
+        dy, x, w, b, mean.contiguous(), rstd.contiguous(), T, num_groups, act, code, pdt, spec,
+        _params(C, clamp_value, batch_divisor, noise), need_dx, need_dw, return_norms)
+    _lib.check(st, "fdp_group_norm_bwd")
+    return (dx, dgamma, dbeta, ng, nb) if return_norms else (dx, dgamma, dbeta)
+
+
 def _ln_identity_stats(rows, device):
     return (torch.zeros(rows, dtype=torch.float32, device=device),
             torch.ones(rows, dtype=torch.float32, device=device))

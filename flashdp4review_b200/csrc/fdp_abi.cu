@@ -105,6 +105,33 @@ int check_params(const fdp_dp_params* p) {
   return FDP_OK;
 }
 
+// (null: no dropout)
+int check_dropout(const fdp_dropout_params* p) {
+  if (p == nullptr) return FDP_OK;
+  if (!(p->p >= 0.0 && p->p <= 1.0)) return FDP_ERR_ARG;
+  if (p->offset >= 1ull << 60) return FDP_ERR_ARG;
+  return FDP_OK;
+}
+int check_group_norm(int B, int T, int C, int G, int activation, int dtype, int param_dtype, const fdp_dropout_params* drop) {
+  if (B <= 0 || T <= 0 || C <= 0 || G <= 0 || activation < FDP_ACT_NONE || activation > FDP_ACT_GELU_TANH) return FDP_ERR_ARG;
+  if (!valid_dtype(dtype) || !valid_dtype(param_dtype)) return FDP_ERR_DTYPE;
+  if (C % G != 0 || C > GN_MAX_CHANNELS || static_cast<long long>(B) * T >= (1ll << 31) / 2) return FDP_ERR_SHAPE;
+  return check_dropout(drop);
+}
+// workspace of fdp_group_norm_bwd
+struct GnBwdWs { float *sumsq, *factors, *gpart, *part; size_t bytes; };
+GnBwdWs gn_bwd_ws(void* base, int B, int T, int C, int G) {
+  GnBwdWs w;
+  const size_t chunks = gn_plan(B, T, C).chunks;
+  Carver c(base);
+  w.sumsq = c.take<float>(static_cast<size_t>(2) * B * ln_sumsq_parts(C));
+  w.factors = c.take<float>(static_cast<size_t>(2) * B);
+  w.gpart = c.take<float>(2 * B * chunks * G);
+  w.part = c.take<float>(2 * B * chunks * C);
+  w.bytes = c.off;
+  return w;
+}
+
 // workspace of fdp_linear_wgrad: [status word | norms | factors | partials | tensor-core extra]
 struct WgradWs {
   int* status; float* norms; float* factors; float* partials; void* tc_extra;
@@ -794,6 +821,78 @@ int fdp_layernorm_bwd_saturate(const void* dy, const void* x, const float* mean,
   float* db_buf = dw_buf + static_cast<size_t>(ln_saturate_groups(rows, d)) * d;
   ln_saturate(dy, x, mean, rstd, dw_buf, db_buf, dgamma, dbeta, rows, d, dtype, param_dtype, C, clamp_value,
               static_cast<cudaStream_t>(stream));
+  FDP_LAUNCH_OK();
+  return FDP_OK;
+}
+
+int fdp_dropout(const void* x, const void* residual, void* y, size_t n, int dtype, const fdp_dropout_params* p, fdp_stream_t stream) {
+  NvtxRange nvtx_range("fdp_dropout");
+  if (p == nullptr) return FDP_ERR_ARG;
+  if (!valid_dtype(dtype)) return FDP_ERR_DTYPE;
+  int st = check_dropout(p);
+  if (st != FDP_OK) return st;
+  if (n == 0) return FDP_OK;
+  if (x == nullptr || y == nullptr) return FDP_ERR_ARG;
+  if ((st = current_device_ok()) != FDP_OK) return st;
+  dropout(x, residual, y, n, dtype, p, static_cast<cudaStream_t>(stream));
+  FDP_LAUNCH_OK();
+  return FDP_OK;
+}
+
+size_t fdp_group_norm_fwd_workspace_bytes(int B, int T, int C, int G) {
+  if (B <= 0 || T <= 0 || C <= 0 || G <= 0) return 0;
+  return sizeof(float) * 2 * B * static_cast<size_t>(gn_plan(B, T, C).chunks) * G;
+}
+
+int fdp_group_norm_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd, int B, int T, int C, int G,
+                       float eps, int activation, int dtype, int param_dtype, const fdp_dropout_params* drop, void* workspace,
+                       size_t workspace_bytes, fdp_stream_t stream) {
+  NvtxRange nvtx_range("fdp_group_norm_fwd");
+  if (x == nullptr || y == nullptr || mean == nullptr || rstd == nullptr || (gamma == nullptr) != (beta == nullptr)) return FDP_ERR_ARG;
+  int st = check_group_norm(B, T, C, G, activation, dtype, param_dtype, drop);
+  if (st != FDP_OK) return st;
+  if ((st = current_device_ok()) != FDP_OK) return st;
+  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < fdp_group_norm_fwd_workspace_bytes(B, T, C, G)) return FDP_ERR_WORKSPACE;
+  GnArgs a{};
+  a.x = x; a.gamma = gamma; a.beta = beta; a.y = y; a.mean = mean; a.rstd = rstd;
+  a.B = B; a.T = T; a.C = C; a.G = G; a.act = activation; a.pdt = param_dtype; a.eps = eps; a.drop = drop; a.workspace = workspace;
+  if ((st = gn_fwd(a, dtype, static_cast<cudaStream_t>(stream))) != FDP_OK) return st;
+  FDP_LAUNCH_OK();
+  return FDP_OK;
+}
+
+size_t fdp_group_norm_bwd_workspace_bytes(int B, int T, int C, int G) {
+  if (B <= 0 || T <= 0 || C <= 0 || G <= 0) return 0;
+  return gn_bwd_ws(nullptr, B, T, C, G).bytes;
+}
+
+int fdp_group_norm_bwd(const void* dy, const void* x, const void* gamma, const void* beta, const float* mean, const float* rstd, void* dx,
+                       void* dgamma, void* dbeta, float* norms_gamma, float* norms_beta, int B, int T, int C, int G, int activation,
+                       int dtype, int param_dtype, const fdp_dropout_params* drop, const fdp_dp_params* p, void* workspace,
+                       size_t workspace_bytes, fdp_stream_t stream) {
+  NvtxRange nvtx_range("fdp_group_norm_bwd");
+  if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || (gamma == nullptr) != (beta == nullptr) ||
+      (dx == nullptr && dgamma == nullptr) || (dgamma == nullptr) != (dbeta == nullptr) || (dgamma != nullptr && gamma == nullptr))
+    return FDP_ERR_ARG;
+  int st = check_group_norm(B, T, C, G, activation, dtype, param_dtype, drop);
+  if (st != FDP_OK) return st;
+  if ((st = check_params(p)) != FDP_OK) return st;
+  if ((st = current_device_ok()) != FDP_OK) return st;
+  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < fdp_group_norm_bwd_workspace_bytes(B, T, C, G)) return FDP_ERR_WORKSPACE;
+  const GnBwdWs w = gn_bwd_ws(workspace, B, T, C, G);
+  const int chunks = gn_plan(B, T, C).chunks;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  GnArgs a{};
+  a.x = x; a.dy = dy; a.gamma = gamma; a.beta = beta; a.dx = dx;
+  a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
+  a.B = B; a.T = T; a.C = C; a.G = G; a.act = activation; a.pdt = param_dtype; a.drop = drop;
+  if ((st = gn_bwd(a, dtype, w.part, w.gpart, s)) != FDP_OK) return st;
+  if (dgamma != nullptr) {
+    const int div = p->batch_divisor > 0 ? p->batch_divisor : B;
+    ln_psgrad_reduce(w.part, w.sumsq, B, chunks, C, s);
+    ln_clip_finalize(w.part, w.sumsq, ln_sumsq_parts(C), p->C, p->clamp_value, w.factors, norms_gamma, norms_beta, dgamma, dbeta, B, chunks, C,
+                     param_dtype, 1.0f / static_cast<float>(div), make_noise_key(p, p->param_id), make_noise_key(p, p->param_id2), s);
+  }
   FDP_LAUNCH_OK();
   return FDP_OK;
 }

@@ -36,6 +36,11 @@ struct Abi {
   decltype(&fdp_layernorm_fwd) layernorm_fwd;
   decltype(&fdp_layernorm_bwd_workspace_bytes) layernorm_bwd_workspace_bytes;
   decltype(&fdp_layernorm_bwd) layernorm_bwd;
+  decltype(&fdp_dropout) dropout;
+  decltype(&fdp_group_norm_fwd_workspace_bytes) group_norm_fwd_workspace_bytes;
+  decltype(&fdp_group_norm_fwd) group_norm_fwd;
+  decltype(&fdp_group_norm_bwd_workspace_bytes) group_norm_bwd_workspace_bytes;
+  decltype(&fdp_group_norm_bwd) group_norm_bwd;
 } abi;
 
 void bind(const std::map<std::string, uint64_t>& fns) {
@@ -45,6 +50,9 @@ void bind(const std::map<std::string, uint64_t>& fns) {
   FDP_BIND(linear_bwd_workspace_bytes); FDP_BIND(linear_bwd);
   FDP_BIND(linear_dgrad_workspace_bytes); FDP_BIND(linear_dgrad); FDP_BIND(linear_fwd);
   FDP_BIND(layernorm_fwd); FDP_BIND(layernorm_bwd_workspace_bytes); FDP_BIND(layernorm_bwd);
+  FDP_BIND(dropout);
+  FDP_BIND(group_norm_fwd_workspace_bytes); FDP_BIND(group_norm_fwd);
+  FDP_BIND(group_norm_bwd_workspace_bytes); FDP_BIND(group_norm_bwd);
 #undef FDP_BIND
 }
 
@@ -308,6 +316,79 @@ py::tuple layernorm_bwd(const Tensor& dy, const Tensor& x, const Tensor& w, cons
   return py::make_tuple(r.st, r.dx, r.dgamma, r.dbeta, r.ng, r.nb);
 }
 
+// (p, seed, offset, stream id, step, step counter or None), or None
+std::optional<fdp_dropout_params> drop_params(const py::object& o) {
+  if (o.is_none()) return std::nullopt;
+  const py::tuple t = py::reinterpret_borrow<py::tuple>(o);
+  fdp_dropout_params d{};
+  d.p = t[0].cast<double>(); d.seed = t[1].cast<uint64_t>(); d.offset = t[2].cast<uint64_t>();
+  d.stream_id = t[3].cast<uint32_t>(); d.step = t[4].cast<uint32_t>();
+  d.step_device = t[5].is_none() ? nullptr : reinterpret_cast<decltype(d.step_device)>(t[5].cast<uint64_t>());
+  return d;
+}
+
+py::tuple dropout(const Tensor& x, const OptTensor& residual, const OptTensor& out, int dt, const py::object& spec) {
+  const fdp_dropout_params d = drop_params(spec).value();
+  if (residual.has_value() && (residual->device() != x.device() || residual->sizes() != x.sizes())) refuse("residual does not fit the input", *residual);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor y = out.has_value() ? *out : new_tensor(x, x.sizes(), x.scalar_type());
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = abi.dropout(ptr(x), ptr(residual), ptr(y), static_cast<size_t>(x.numel()), dt, &d, stream(x));
+  }
+  return py::make_tuple(st, y);
+}
+
+// parameters (both or neither) and statistics of a group norm over x [B, ..., C]
+void check_group_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, const OptTensor& mean, const OptTensor& rstd, const OptTensor& dy, int64_t G) {
+  const int64_t C = x.size(-1), B = x.size(0);
+  for (const OptTensor& t : {w, b})
+    if (t.has_value() && (t->device() != x.device() || t->numel() != C)) refuse("group norm: parameters do not fit the input's channels", *t);
+  for (const OptTensor& t : {mean, rstd})
+    if (t.has_value() && (t->device() != x.device() || t->numel() != B * G || t->scalar_type() != at::kFloat)) refuse("group norm: statistics do not fit the input", *t);
+  if (dy.has_value() && (dy->device() != x.device() || dy->sizes() != x.sizes())) refuse("group norm: grad_output does not fit the input", *dy);
+}
+
+py::tuple group_norm_fwd(const Tensor& x, const OptTensor& w, const OptTensor& b, int T, int G, double eps, int act, int dt, int pdt, const py::object& spec) {
+  check_group_norm(x, w, b, {}, {}, {}, G);
+  const auto d = drop_params(spec);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int B = static_cast<int>(x.size(0)), C = static_cast<int>(x.size(-1));
+  const Tensor y = new_tensor(x, x.sizes(), x.scalar_type());
+  const Tensor mean = new_tensor(x, {B, G}, at::kFloat), rstd = new_tensor(x, {B, G}, at::kFloat);
+  const Tensor ws = workspace(x, abi.group_norm_fwd_workspace_bytes(B, T, C, G));
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = abi.group_norm_fwd(ptr(x), ptr(w), ptr(b), ptr(y), static_cast<float*>(ptr(mean)), static_cast<float*>(ptr(rstd)), B, T, C, G,
+                            static_cast<float>(eps), act, dt, pdt, d ? &*d : nullptr, ptr(ws), ws.numel(), stream(x));
+  }
+  return py::make_tuple(st, y, mean, rstd);
+}
+
+py::tuple group_norm_bwd(const Tensor& dy, const Tensor& x, const OptTensor& w, const OptTensor& b, const Tensor& mean, const Tensor& rstd, int T, int G,
+                         int act, int dt, int pdt, const py::object& spec, const py::tuple& p, bool need_dx, bool need_dw, bool want_norms) {
+  check_group_norm(x, w, b, mean, rstd, dy, G);
+  const fdp_dp_params q = params(p);
+  const auto d = drop_params(spec);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int B = static_cast<int>(x.size(0)), C = static_cast<int>(x.size(-1));
+  OptTensor dx, dgamma, dbeta, ng, nb;
+  if (need_dx) dx = new_tensor(x, x.sizes(), x.scalar_type());
+  if (need_dw) { dgamma = new_tensor(x, {C}, w->scalar_type()); dbeta = new_tensor(x, {C}, b->scalar_type()); }
+  if (need_dw && want_norms) { ng = new_tensor(x, {B}, at::kFloat); nb = new_tensor(x, {B}, at::kFloat); }
+  const Tensor ws = workspace(x, abi.group_norm_bwd_workspace_bytes(B, T, C, G));
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = abi.group_norm_bwd(ptr(dy), ptr(x), ptr(w), ptr(b), static_cast<const float*>(ptr(mean)), static_cast<const float*>(ptr(rstd)), ptr(dx),
+                            ptr(dgamma), ptr(dbeta), static_cast<float*>(ptr(ng)), static_cast<float*>(ptr(nb)), B, T, C, G, act, dt, pdt,
+                            d ? &*d : nullptr, &q, ptr(ws), ws.numel(), stream(x));
+  }
+  return py::make_tuple(st, dx, dgamma, dbeta, ng, nb);
+}
+
 // ---- the layers' autograd nodes --------------------------------------------------------------------------------------
 // What the Function classes of layers/*.py do, without a Python frame per tensor operation: a pass of a small layer is
 // bound by the host, and of its 120 to 160 us those classes took a third.  Choices and noise bookkeeping stay in
@@ -543,6 +624,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_fwd", &linear_fwd);
   m.def("layernorm_fwd", &layernorm_fwd);
   m.def("layernorm_bwd", &layernorm_bwd);
+  m.def("dropout", &dropout);
+  m.def("group_norm_fwd", &group_norm_fwd);
+  m.def("group_norm_bwd", &group_norm_bwd);
   m.def("bind_layers", &bind_layers);
   m.def("dp_linear", &dp_linear);
   m.def("dp_layernorm", &dp_layernorm);

@@ -103,6 +103,27 @@ bool tc_split_stats_ok(const void* G, int n_out);
 int tc_split_stats(const void* G, void* dst, float* colsum_part, float* sq_part, int B, int T, int n_out, int planes,
                    const GstatsPlan& pl, cudaStream_t s, unsigned* maximum = nullptr);
 
+// ---- dropout (fdp_dropout.cuh) ----------------------------------------------------------------------
+// y = keep * x / (1 - p) (+ residual) over n elements; y may be x or residual
+void dropout(const void* x, const void* residual, void* y, size_t n, int dt, const fdp_dropout_params* p, cudaStream_t s);
+
+// ---- group norm, channels last ------------------------------------------------------------------------
+constexpr int GN_MAX_CHANNELS = 8192;
+struct GnPlan { bool vec; int rows_per_chunk, chunks; };
+GnPlan gn_plan(int B, int T, int C);
+struct GnArgs {
+  const void *x, *dy, *gamma, *beta;     // gamma, beta may be null (one and zero)
+  void *y, *dx;                          // dx may be null
+  float *mean, *rstd;                    // [B, G]
+  int B, T, C, G, act, pdt;
+  float eps;
+  const fdp_dropout_params* drop;        // null: none
+  void* workspace;                       // forward: float2[B, chunks, G]
+};
+int gn_fwd(const GnArgs& a, int dt, cudaStream_t s);
+// part: [2][B][chunks][C] (of dgamma, then of dbeta), what ln_psgrad_reduce takes; gpart: float2[B, chunks, G]
+int gn_bwd(const GnArgs& a, int dt, float* part, float* gpart, cudaStream_t s);
+
 // ---- LayerNorm -----------------------------------------------------------------------------------
 struct LnPlan { int tpr, cpt, cw, rows_per_block, chunks; bool vec; };
 LnPlan ln_plan(int B, int T, int d, int dt);

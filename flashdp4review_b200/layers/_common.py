@@ -50,6 +50,22 @@ def dp_scalars(local_batch, noise_multiplier, param_id, step, param_id2=0):
                                    step_device=runtime.device_noise_counter() if std != 0.0 else None)
 
 
+def dropout_spec(p, stream_id, x):
+    """The mask of one forward pass of a dropout over as many elements as `x` has, for its backward to draw again.
+
+    The seed is drawn from torch's CPU generator, which torch.utils.checkpoint restores before it runs a pass again: a count
+    of the layer's own would give the recomputed pass another mask than the one whose output the rest of the network has
+    seen.  A data-parallel rank's elements are numbered behind those of the ranks before it.  With the device counter on
+    (a step captured in a graph) the step is its value now, copied on the stream, since it may have moved on by the time the
+    backward runs."""
+    counter = runtime.device_noise_counter(x.device) if x.is_cuda else None
+    if counter is None and x.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a captured dropout would draw the same mask on every replay: call use_device_noise_step() first")
+    return ops.DropoutSpec(p=p, seed=int(torch.randint(-2 ** 63, 2 ** 63 - 1, (), device="cpu")) & (2 ** 64 - 1), stream_id=stream_id,
+                           offset=runtime.data_parallel()[0] * ((x.numel() + 7) // 8),
+                           step_device=None if counter is None else counter.clone())
+
+
 def direct_grad_target(param):
     """The bucket slice a DP weight gradient may be written into directly, or None.
 

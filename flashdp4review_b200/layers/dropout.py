@@ -1,0 +1,67 @@
+"""DPDropout: nn.Dropout whose mask is drawn from a counter-based generator in the kernels, forward and backward, and never
+stored; the residual sum behind it is part of the call.  No counterpart in the reference, whose models use nn.Dropout.
+"""
+import torch
+import torch.nn as nn
+from torch.autograd.function import Function, once_differentiable
+
+from .. import runtime
+from ..core import ops
+from ._common import dropout_spec
+
+
+def _storage_order(x):
+    """The axes of a dense tensor from the slowest to the fastest, so that channels-last storage is walked as it lies."""
+    order = sorted(range(x.dim()), key=lambda d: (-x.stride(d), d))
+    return order if x.permute(order).is_contiguous() else list(range(x.dim()))
+
+
+class _DropoutFunc(Function):
+    @staticmethod
+    def forward(ctx, input, residual, spec, inplace):
+        # elements are numbered in the order of the input's storage; the gradient is brought into the same one
+        ctx.order, ctx.spec = _storage_order(input), spec
+        x = input.permute(ctx.order)
+        into = inplace and x.is_contiguous()
+        y = ops.dropout(x, spec, residual=None if residual is None else residual.permute(ctx.order), out=x if into else None)
+        y = y.permute(_inverse(ctx.order))
+        if not inplace:
+            return y
+        if not into:
+            input.copy_(y)
+        ctx.mark_dirty(input)
+        return input
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = ops.dropout_backward(grad_output.permute(ctx.order), ctx.spec).permute(_inverse(ctx.order))
+        return dx, grad_output if ctx.needs_input_grad[1] else None, None, None
+
+
+def _inverse(order):
+    inverse = [0] * len(order)
+    for i, d in enumerate(order):
+        inverse[d] = i
+    return inverse
+
+
+class DPDropout(nn.Dropout):
+    """`forward(input)` drops as nn.Dropout does; `forward(input, residual)` adds `residual` in the same kernel.  In
+    evaluation mode, and for p = 0, the input (or the sum) comes back.  The mask's seed is drawn from torch's CPU generator:
+    torch.manual_seed repeats a run, and torch.utils.checkpoint, which restores that generator, draws a recomputed pass's
+    mask again.  Data-parallel ranks draw for their own shards.  In a captured step use_device_noise_step() has to be on
+    (every replay then draws anew), else the call is refused."""
+
+    def __init__(self, p: float = 0.5, inplace: bool = False):
+        super().__init__(p, inplace)
+        self._stream_id = runtime.next_param_id()
+
+    def forward(self, input, residual=None):
+        if not self.training or self.p == 0.0:
+            return input if residual is None else input + residual
+        if self.inplace and residual is not None:
+            raise RuntimeError("dropout in place takes no residual")
+        return _DropoutFunc.apply(input, residual, dropout_spec(self.p, self._stream_id, input), self.inplace)

@@ -33,8 +33,9 @@ extern "C" {
  * 3: fdp_dp_params.step_device (appended; earlier fields keep their offsets); FDP_FP32_TENSOR also
  *    accepted in the dtype of fdp_linear_dgrad / fdp_linear_fwd.
  * 4: FDP_FP32_WIDE, fdp_linear_bwd.
- * 5: FDP_KEEP_PRODUCTS, FDP_FP32_WIDE_GEMM, FDP_GEMM_SPLIT_K, FDP_PAD_16BIT. */
-#define FDP_ABI_VERSION 5
+ * 5: FDP_KEEP_PRODUCTS, FDP_FP32_WIDE_GEMM, FDP_GEMM_SPLIT_K, FDP_PAD_16BIT.
+ * 6: fdp_group_norm_fwd / _bwd, fdp_dropout. */
+#define FDP_ABI_VERSION 6
 
 typedef void* fdp_stream_t; /* a cudaStream_t */
 
@@ -304,6 +305,49 @@ int fdp_layernorm_saturate_groups(int rows, int d);
 int fdp_layernorm_bwd_saturate(const void* dy, const void* x, const float* mean, const float* rstd, void* dgamma,
                                void* dbeta, int rows, int d, int dtype, int param_dtype, float C, float clamp_value,
                                void* workspace, size_t workspace_bytes, fdp_stream_t stream);
+
+/* ---- dropout without a stored mask ------------------------------------------------------------------
+ * No counterpart in the reference (its models use torch.nn.Dropout beside the DP layers).
+ *   y[i] = (keep(i) ? x[i] / (1 - p) : 0) + residual[i]   over n elements in row-major order, each rounded once.
+ * The backward is the same call on the gradient, without a residual.  keep(i) is a function of the parameters and i alone:
+ * element i is number i % 8 of group offset + i / 8; the group's Philox4x32-10 draw (key: seed's low word, its high word ^
+ * 0x44524F50; counter: group's low word, high word, stream_id, step) gives each number 16 bits, word i % 8 / 2, low half
+ * first; the same 16 bits of the draw with bit 63 of the group set lie below them; the element is dropped if the 32 bits are
+ * less than round(p 2^32).  p = 1 drops everything; a dropped element is 0 whatever x holds.
+ * `offset`, in groups of eight and below 2^60, lets the ranks of a data-parallel job draw apart.  x, residual and y may be
+ * one buffer.  n = 0 is a no-op.
+ */
+typedef struct fdp_dropout_params {
+  double p;                    /* 0 <= p <= 1 */
+  uint64_t seed;
+  uint64_t offset;             /* groups of eight elements */
+  uint32_t stream_id;
+  uint32_t step;
+  const uint32_t* step_device; /* NULL, or a device counter added to `step` when the kernels run */
+} fdp_dropout_params;
+int fdp_dropout(const void* x, const void* residual, void* y, size_t n, int dtype, const fdp_dropout_params* p,
+                fdp_stream_t stream);
+
+/* ---- group norm, channels last, with activation and dropout behind it ---------------------------------
+ * No counterpart in the reference.  Statistics are those of one sample, as per-sample clipping needs.
+ *   x, y [B,T,C] in `dtype`; gamma, beta [C] in `param_dtype`, both or neither NULL (one and zero); mean, rstd float[B,G];
+ *   C a multiple of G, at most 8192.  y = dropout(act(xhat * gamma + beta)), rounded once; drop NULL: no dropout (its
+ *   elements are numbered as those of y).
+ * fdp_group_norm_bwd: dx as autograd's; dgamma / dbeta [C] in `param_dtype` are the per-sample gradients, each clipped by its
+ *   norm, summed over the batch / batch_divisor, plus noise (param_id, param_id2), as in fdp_layernorm_bwd.  dx, the pair
+ *   dgamma / dbeta and the norms (float[B]) may be NULL; beta is read where there is an activation.
+ */
+enum fdp_activation { FDP_ACT_NONE = 0, FDP_ACT_RELU = 1, FDP_ACT_SILU = 2, FDP_ACT_GELU = 3, FDP_ACT_GELU_TANH = 4 };
+size_t fdp_group_norm_fwd_workspace_bytes(int B, int T, int C, int G);
+int fdp_group_norm_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd, int B, int T,
+                       int C, int G, float eps, int activation, int dtype, int param_dtype,
+                       const fdp_dropout_params* drop, void* workspace, size_t workspace_bytes, fdp_stream_t stream);
+size_t fdp_group_norm_bwd_workspace_bytes(int B, int T, int C, int G);
+int fdp_group_norm_bwd(const void* dy, const void* x, const void* gamma, const void* beta, const float* mean,
+                       const float* rstd, void* dx, void* dgamma, void* dbeta, float* norms_gamma, float* norms_beta,
+                       int B, int T, int C, int G, int activation, int dtype, int param_dtype,
+                       const fdp_dropout_params* drop, const fdp_dp_params* p, void* workspace, size_t workspace_bytes,
+                       fdp_stream_t stream);
 
 #ifdef __cplusplus
 }
