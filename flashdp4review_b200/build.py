@@ -13,7 +13,8 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libfdp_b200.so")
 HOST_LIB = os.path.join(PKG, "_fdp_host.so")
 HOST_SOURCE = os.path.join(CSRC, "fdp_host.cpp")
-SOURCES = ["fdp_abi.cu", "fdp_simt.cu", "fdp_layernorm.cu", "fdp_tc.cu", "fdp_static.cu", "fdp_dropout.cu", "fdp_groupnorm.cu"]
+SOURCES = ["fdp_abi.cu", "fdp_simt.cu", "fdp_layernorm.cu", "fdp_tc.cu", "fdp_static.cu", "fdp_dropout.cu", "fdp_groupnorm.cu",
+           "fdp_fp8.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 

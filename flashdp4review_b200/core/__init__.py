@@ -4,5 +4,6 @@ from .ops import (  # noqa: F401
     mm_fused,
     dp_linear_weight_grad, dp_bias_grad, dp_layernorm_backward, linear_input_grad, linear_forward,
     DropoutSpec, dropout, dropout_backward, group_norm_forward, dp_group_norm_backward,
+    Fp8Weight, fp8_quantize, fp8_quantize_weight, fp8_linear_forward, fp8_linear_input_grad,
     RuntimeAutoTuner, NoiseSpec, noise_std,
 )

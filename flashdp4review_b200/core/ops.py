@@ -536,6 +536,72 @@ def dp_group_norm_backward(grad_output, input, weight, bias, mean, rstd, num_gro
     return (dx, dgamma, dbeta, ng, nb) if return_norms else (dx, dgamma, dbeta)
 
 
+# ------------------------------------------------------------------------------------------------
+# products in 8-bit floating point
+# ------------------------------------------------------------------------------------------------
+@dataclass
+class Fp8Weight:
+    """A weight in e4m3 with one power-of-two scale for each block of 128 x 128, as it lies and transposed: [out, in] (layout
+    "out_in") or [in, out] ("in_out").  What it stands for is values * scales, block by block."""
+    values: object        # float8_e4m3fn [r, c]
+    values_t: object      # [c, r]
+    scales: object        # float32 [ceil(r / 128), ceil(c / 128)]
+    layout: str = "out_in"
+
+
+def fp8_quantize(input):
+    """`input` (..., K) in e4m3 with one power-of-two scale for each row and 128 columns: (values (rows, K), scales
+    (rows, ceil(K / 128))).  What is not finite becomes a NaN."""
+    host = _lib.host()
+    _require_cuda(input)
+    code = _dt(input.dtype)
+    if input.dim() < 1 or input.numel() == 0:
+        raise RuntimeError(f"nothing to quantise in a tensor of shape {tuple(input.shape)}")
+    st, q, scales = host.fp8_quantize(input.reshape(-1, input.shape[-1]).contiguous(), code)
+    _lib.check(st, "fdp_fp8_quantize")
+    return q, scales.t()
+
+
+def fp8_quantize_weight(weight, layout="out_in"):
+    """The Fp8Weight of a weight (out, in) or, with layout "in_out", (in, out): to be made once per change of the weight and
+    used in the forward product and in the input gradient."""
+    host = _lib.host()
+    _require_cuda(weight)
+    code = _dt(weight.dtype)
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise RuntimeError(f"expected a weight with two dimensions, got {tuple(weight.shape)}")
+    if layout not in ("out_in", "in_out"):
+        raise ValueError(f"layout must be 'out_in' or 'in_out', got {layout!r}")
+    st, q, qt, scales = host.fp8_quantize_weight(weight.contiguous(), code)
+    _lib.check(st, "fdp_fp8_quantize_weight")
+    return Fp8Weight(q, qt, scales, layout)
+
+
+def _fp8_product(x, weight, bias, transposed, out_dtype):
+    host = _lib.host()
+    _require_cuda(x, weight.values, bias)
+    code = _dt(x.dtype)
+    if x.numel() == 0:
+        raise RuntimeError(f"product with an empty operand {tuple(x.shape)}")
+    w, scales = (weight.values_t, weight.scales.t()) if transposed else (weight.values, weight.scales)
+    b = None if bias is None else bias.to(x.dtype).contiguous()
+    st, y = host.fp8_matmul(x.contiguous(), w, scales, b, code, _dt(out_dtype or x.dtype))
+    _lib.check(st, "fdp_fp8_matmul")
+    return y
+
+
+def fp8_linear_forward(input, weight, bias=None, out_dtype=None):
+    """input @ weight.t() + bias (weight an Fp8Weight; input @ weight + bias for layout "in_out") in e4m3: the input is
+    quantised as by `fp8_quantize` within the call, so its rows (samples) stay apart; products are accumulated in fp32 and
+    rounded once to `out_dtype` (default: the input's)."""
+    return _fp8_product(input, weight, bias, weight.layout == "in_out", out_dtype)
+
+
+def fp8_linear_input_grad(grad_output, weight, out_dtype=None):
+    """grad_output @ weight (weight.t() for layout "in_out") in e4m3, as `fp8_linear_forward`."""
+    return _fp8_product(grad_output, weight, None, weight.layout != "in_out", out_dtype)
+
+
 def _ln_identity_stats(rows, device):
     return (torch.zeros(rows, dtype=torch.float32, device=device),
             torch.ones(rows, dtype=torch.float32, device=device))

@@ -1,0 +1,614 @@
+// Products in 8-bit floating point (e4m3) with one scale for each block of 128 numbers of the contraction.
+//
+//   Y[m, n] = sum_kb s_a[m, kb] * s_w[n / 128, kb] * sum_{k in kb} q_a[m, k] q_w[n, k]  (+ bias[n])
+//
+// Activations and gradients have a scale for each row and 128 columns, so that no number of one sample depends on another
+// sample's (per-sample clipping needs that); weights one for each 128 x 128 block, which serves both the forward product
+// and the input gradient.  Scales are powers of two, the smallest that brings a block's largest finite magnitude to at
+// most 448: dividing by one and multiplying by two of them is exact, so the only roundings are those to e4m3, those of
+// the accumulation and the last one.  A number that is not finite becomes a NaN (e4m3 has no infinity).
+//
+// The matrix instruction accumulates one K block (128 numbers, 128 bytes a row: one stage of the ring) in TMEM; the
+// epilogue warps then add it, times the two scales, to fp32 registers, while the next block is multiplied into another
+// accumulator.
+#include <cuda_fp8.h>
+
+#include "fdp_async.cuh"
+#include "fdp_kernels.h"
+#include "fdp_tcgen05.cuh"
+#include "fdp_vec8.cuh"
+
+namespace fdp {
+namespace {
+
+// ---- quantisation -----------------------------------------------------------------------------------
+// bits of |v|, 0 for what is not finite
+__device__ __forceinline__ uint32_t finite_magnitude(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+  return b < 0x7F800000u ? b : 0u;
+}
+// exponent k of the smallest power of two with amax <= 448 * 2^k (448 = 1.75 * 2^8); 0 for a block of zeros; not below -126,
+// so that 2^k and 2^-k are both normal numbers
+__device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
+  if (amax_bits == 0) return 0;
+  const int k = static_cast<int>(amax_bits >> 23) - 127 - ((amax_bits & 0x7FFFFFu) <= 0x600000u ? 8 : 7);
+  return k < -126 ? -126 : k;
+}
+__device__ __forceinline__ float power_of_two(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }
+// eight numbers times 2^-k as e4m3 (round to nearest even; nothing saturates: the block's largest is at most 448)
+__device__ __forceinline__ uint2 to_e4m3x8(const float f[8], float inv) {
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    w[h] = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float a = f[4 * h + 2 * j], b = f[4 * h + 2 * j + 1];
+      if ((__float_as_uint(a) & 0x7F800000u) == 0x7F800000u) a = __uint_as_float(0x7FC00000u);
+      if ((__float_as_uint(b) & 0x7F800000u) == 0x7F800000u) b = __uint_as_float(0x7FC00000u);
+      w[h] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3)) << (16 * j);
+    }
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// eight numbers of a row from column `col` on; what lies past the row's end is 0
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_row8(const T* row, int col, int cols, float f[8]) {
+  if (VEC) {
+    if (col < cols) { unpack8(load8(row + col), f); return; }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = 0.f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = col + e < cols ? to_f32<T>(row[col + e]) : 0.f;
+  }
+}
+
+// Rows: a half warp takes 128 columns of a row, a block 16 rows x QKB blocks of columns.  HBM-bound.
+constexpr int QKB = 4;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) fp8_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales, int rows, int cols,
+                                                       int pitch, int kblocks, int row_tiles) {
+  __shared__ float s_scale[QKB][16];
+  const int hw = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const int r0 = (blockIdx.x % row_tiles) * 16, kb0 = (blockIdx.x / row_tiles) * QKB;
+  const int row = r0 + hw;
+  pdl_trigger();
+  float f[QKB][8];
+#pragma unroll
+  for (int i = 0; i < QKB; ++i) {
+    const int kb = kb0 + i;
+    if (row < rows && kb < kblocks) load_row8<T, VEC>(x + static_cast<size_t>(row) * cols, kb * 128 + l * 8, cols, f[i]);
+    else
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[i][e] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < QKB; ++i) {
+    const int col = (kb0 + i) * 128 + l * 8;
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, finite_magnitude(f[i][e]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const int k = scale_exponent(m);
+    const uint2 w = to_e4m3x8(f[i], power_of_two(-k));
+    if (row < rows && col < pitch) *reinterpret_cast<uint2*>(q + static_cast<size_t>(row) * pitch + col) = w;
+    if (l == 0) s_scale[i][hw] = power_of_two(k);
+  }
+  __syncthreads();
+  if (threadIdx.x < QKB * 16) {
+    const int i = threadIdx.x >> 4, r = threadIdx.x & 15;
+    if (kb0 + i < kblocks && r0 + r < rows) scales[static_cast<size_t>(kb0 + i) * rows + r0 + r] = s_scale[i][r];
+  }
+}
+
+// 4 x 4 bytes transposed: out[j] holds byte j of in[0..3]
+__device__ __forceinline__ void transpose4(const uint32_t in[4], uint32_t out[4]) {
+  const uint32_t a = __byte_perm(in[0], in[1], 0x5140), b = __byte_perm(in[2], in[3], 0x5140);   // bytes 0 and 1 of the pairs
+  const uint32_t c = __byte_perm(in[0], in[1], 0x7362), d = __byte_perm(in[2], in[3], 0x7362);   // bytes 2 and 3
+  out[0] = __byte_perm(a, b, 0x5410);
+  out[1] = __byte_perm(a, b, 0x7632);
+  out[2] = __byte_perm(c, d, 0x5410);
+  out[3] = __byte_perm(c, d, 0x7632);
+}
+// Weights: one block a 128 x 128 block, written as it lies and transposed (both products contract over adjacent bytes).  A
+// half warp holds eight rows of it, a thread 8 x 8 numbers, whose bytes it transposes in registers.
+constexpr int WT_PITCH = 128 + 16;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) fp8_weight_kernel(const T* __restrict__ w, uint8_t* __restrict__ q, uint8_t* __restrict__ qt,
+                                                         float* __restrict__ scales, int rows, int cols, int pitch, int pitch_t, int col_blocks) {
+  __shared__ __align__(16) uint8_t tile[128 * WT_PITCH];
+  __shared__ uint32_t red[8];
+  const int hw = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
+  const int r0 = rb * 128 + hw * 8, c = cb * 128 + l * 8;
+  pdl_trigger();
+  float f[8][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (r0 + i < rows) load_row8<T, VEC>(w + static_cast<size_t>(r0 + i) * cols, c, cols, f[i]);
+    else
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[i][e] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, finite_magnitude(f[i][e]));
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, red[i]);
+  const int k = scale_exponent(m);
+  const float inv = power_of_two(-k);
+  if (threadIdx.x == 0) scales[blockIdx.x] = power_of_two(k);
+  uint2 b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    b[i] = to_e4m3x8(f[i], inv);
+    if (r0 + i < rows && c < pitch) *reinterpret_cast<uint2*>(q + static_cast<size_t>(r0 + i) * pitch + c) = b[i];
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {          // columns 4 half .. 4 half + 3 of the thread's eight
+    uint32_t lo[4], hi[4], in[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) in[i] = half ? b[i].y : b[i].x;
+    transpose4(in, lo);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) in[i] = half ? b[4 + i].y : b[4 + i].x;
+    transpose4(in, hi);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint2*>(tile + (l * 8 + half * 4 + j) * WT_PITCH + hw * 8) = make_uint2(lo[j], hi[j]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int piece = threadIdx.x + i * 256, tc = piece >> 3, tr = (piece & 7) * 16;
+    if (cb * 128 + tc < cols && rb * 128 + tr < pitch_t)
+      *reinterpret_cast<uint4*>(qt + static_cast<size_t>(cb * 128 + tc) * pitch_t + rb * 128 + tr) = *reinterpret_cast<const uint4*>(tile + tc * WT_PITCH + tr);
+  }
+}
+
+// ---- the product --------------------------------------------------------------------------------------
+// A persistent, warp-specialised kernel: warp 0 copies (TMA, 128-byte swizzle), warp 1 issues the matrix instructions and owns
+// TMEM, warps 2 to 9 add up and store, two on each TMEM lane quarter.  CTAS = 2: a cluster of two CTAs works on 256 rows, each
+// loads its 128 rows of A and half of the tile's columns of B, the even one issues for both.  Both operands are K-major.
+// One commit a stage, on a barrier of the stage: the epilogue waits for it to read the accumulator, the copying warp to fill
+// the stage again.  (Neither can be a whole turn of the ring behind: the copies wait for it, and the matrix warp waits for
+// the epilogue at most ACCS stages on.)
+constexpr int F8_BM = 128, F8_THREADS = 320, F8_RING = 192 * 1024;
+constexpr int F8_SMEM = F8_RING + 1024 + 8 * BOX_BYTES + 256;
+template <int CTAS, int BN> struct F8Tile {
+  static constexpr int A_BYTES = F8_BM * 128, B_BYTES = BN / CTAS * 128, STG = A_BYTES + B_BYTES;
+  static constexpr int STAGES = F8_RING / STG < 8 ? F8_RING / STG : 8;
+  static constexpr int ACCS = TMEM_COLS / BN < 4 ? TMEM_COLS / BN : 4;
+  static constexpr int WC = BN / 2;          // columns of an epilogue warp
+};
+
+struct Fp8Args {
+  int M, N, kblocks;
+  int tiles_m, tiles_n, m_group, split;
+  const float* sa;                          // [kblocks][M]
+  const float* sw; int sw_n, sw_k;          // scale of (n block, k block) at n * sw_n + k * sw_k
+  void* out; int out_dt; int direct_out;
+  const void* bias; int bias_dt;
+  float* parts;                             // split > 1: [unit][CTA][epilogue warp][WC / 32][1024]
+  int* sticky;
+};
+
+template <int CTAS>
+__device__ __forceinline__ void f8_mma(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 a, {%1, %2};\n\t"
+      "mov.b64 b, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::%7.kind::f8f6f4 [%0], a, b, %5, p;\n\t}"
+      ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "n"(CTAS) : "memory");
+}
+// e4m3 x e4m3 -> fp32, both operands K-major
+__host__ __device__ constexpr uint32_t f8_idesc(int ctas, int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>((F8_BM * ctas) >> 4) << 24);
+}
+
+// rows of a warp's box one by one: an output that the copy engine cannot write
+template <typename T>
+__device__ __forceinline__ void f8_store_rows(T* out, size_t ld, uint32_t box, int rows, int lane, bool in) {
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int r = r0 + k;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[k]) : "r"(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (in && r0 + k < rows) out[static_cast<size_t>(r0 + k) * ld] = from_f32<T>(v[k]);
+  }
+}
+
+template <int CTAS, int BN>
+__global__ void __launch_bounds__(F8_THREADS, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmOut,
+                const __grid_constant__ Fp8Args args) {
+  using L = F8Tile<CTAS, BN>;
+  constexpr int NST = L::STAGES, NACC = L::ACCS, WC = L::WC, STG = L::STG;
+  static_assert(NACC < NST, "one barrier a stage serves the copies and the epilogue");
+  const uint32_t cta_rank = CTAS == 2 ? cluster_ctarank() : 0u;
+  const bool is_leader = cta_rank == 0;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw), base = (raw_addr + 1023u) & ~1023u;
+  const uint32_t boxes = base + F8_RING, bar_base = boxes + 8 * BOX_BYTES;
+  uint8_t* bar_gen = smem_raw + (bar_base - raw_addr);
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto done_bar = [&](int s) { return bar_base + 8u * (8 + s); };
+  auto free_bar = [&](int a) { return bar_base + 8u * (16 + a); };
+  const uint32_t drain_bar = bar_base + 8u * 20;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * 21);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 8 * 21 + 4);
+  const WaitCtx wctx{abort_flag, nullptr, args.sticky, WAIT_LIMIT_CYCLES};
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int units = args.tiles_m * args.tiles_n * args.split;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NST; ++s) { mbar_init(full_bar(s), 1); mbar_init(done_bar(s), 1); }
+    for (int a = 0; a < NACC; ++a) mbar_init(free_bar(a), 8 * CTAS);
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (CTAS == 2) {
+    __syncthreads();
+    cluster_sync_all();      // the peer's barriers must be initialised before anything is signalled across the pair
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::%2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(const_cast<uint32_t*>(tmem_slot))), "r"(TMEM_COLS), "n"(CTAS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::%0.sync.aligned;" ::"n"(CTAS) : "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();
+  pdl_wait();
+  const int wid = blockIdx.x / CTAS, wstep = gridDim.x / CTAS;
+  const uint32_t tmem_base = *tmem_slot;
+
+  // unit -> tile, K blocks.  Tiles are walked in groups of m_group tile rows, so that the CTAs that run together share operands.
+  auto decode = [&](int u, int& m0, int& n0, int& k0, int& k1) {
+    const int tile = u / args.split, part = u - tile * args.split;
+    k0 = static_cast<int>(static_cast<long long>(args.kblocks) * part / args.split);
+    k1 = static_cast<int>(static_cast<long long>(args.kblocks) * (part + 1) / args.split);
+    const int per_group = args.m_group * args.tiles_n;
+    const int g = tile / per_group, r = tile - g * per_group;
+    const int gm = min(args.m_group, args.tiles_m - g * args.m_group);
+    m0 = (g * args.m_group + r % gm) * (F8_BM * CTAS) + static_cast<int>(cta_rank) * F8_BM;
+    n0 = r / gm * BN;
+  };
+
+  if (warp == 0) {
+    // ================= copies =================
+    int stage = 0; uint32_t phase = 0;
+    bool ok = true;
+    for (int u = wid; u < units && ok; u += wstep) {
+      int m0, n0, k0, k1;
+      decode(u, m0, n0, k0, k1);
+      for (int kb = k0; kb < k1; ++kb) {
+        if (!mbar_wait_warp(done_bar(stage), phase ^ 1u, wctx, 21)) { ok = false; break; }
+        if (elect_one()) {
+          const uint32_t sa = base + stage * STG, sb = sa + L::A_BYTES;
+          const uint32_t lbar = CTAS == 1 ? full_bar(stage) : mapa_u32(full_bar(stage), 0);
+          if (is_leader) mbar_expect_tx(full_bar(stage), CTAS * STG);
+          const int nb = n0 + static_cast<int>(cta_rank) * (BN / CTAS);
+          if (CTAS == 1) {
+            tma_load_2d(sa, &tmA, kb * 128, m0, lbar);
+            tma_load_2d(sb, &tmB, kb * 128, nb, lbar);
+          } else {
+            tma_load_2d_pair(sa, &tmA, kb * 128, m0, lbar);
+            tma_load_2d_pair(sb, &tmB, kb * 128, nb, lbar);
+          }
+        }
+        __syncwarp();
+        if (++stage == NST) { stage = 0; phase ^= 1u; }
+      }
+    }
+    if (!ok && lane == 0 && is_leader) {
+      // wait (bounded) for the copies already in flight before the CTA may leave
+      for (int s = 0; s < NST; ++s) {
+        const long long t0 = clock64();
+        const uint32_t ph = (s < stage) ? phase : (phase ^ 1u);
+        while (!mbar_try(full_bar(s), ph) && clock64() - t0 < WAIT_LIMIT_CYCLES / 8) {}
+      }
+    }
+  } else if (warp == 1) {
+    // ================= matrix instructions: the whole warp walks, one elected lane issues =================
+    if (is_leader) {
+      int stage = 0; uint32_t phase = 0;
+      int it = 0;
+      bool ok = true;
+      const Desc a0 = make_desc(base, 0, 1024), b0 = make_desc(base + L::A_BYTES, 0, 1024);
+      for (int u = wid; u < units && ok; u += wstep) {
+        int m0, n0, k0, k1;
+        decode(u, m0, n0, k0, k1);
+        for (int kb = k0; kb < k1; ++kb, ++it) {
+          const int acc = it % NACC;
+          if (!mbar_wait_warp(free_bar(acc), ((it / NACC) & 1u) ^ 1u, wctx, 22) || !mbar_wait_warp(full_bar(stage), phase, wctx, 23)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t so = static_cast<uint32_t>(stage * STG) >> 4;
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)        // 32 numbers, 32 bytes, each
+              f8_mma<CTAS>(tmem_base + acc * BN, a0.lo + so + 2 * k, a0.hi, b0.lo + so + 2 * k, b0.hi, f8_idesc(CTAS, BN), k > 0 ? 1u : 0u);
+            if (CTAS == 1) tc_commit(done_bar(stage)); else tc_commit_pair(done_bar(stage));
+          }
+          __syncwarp();
+          if (++stage == NST) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok && elect_one()) {
+        // let the instructions already issued finish before TMEM is released
+        if (CTAS == 1) tc_commit(drain_bar); else tc_commit_pair(drain_bar);
+        const long long t0 = clock64();
+        while (!mbar_try(drain_bar, 0) && clock64() - t0 < WAIT_LIMIT_CYCLES / 8) {}
+      }
+    }
+  } else {
+    // ================= epilogue =================
+    const int quarter = warp & 3, ew = warp - 2, chalf = ew >> 2;
+    const uint32_t box = boxes + ew * BOX_BYTES;
+    int stage = 0; uint32_t phase = 0;
+    int it = 0;
+    bool ok = true;
+    for (int u = wid; u < units && ok; u += wstep) {
+      int m0, n0, k0, k1;
+      decode(u, m0, n0, k0, k1);
+      const int m = m0 + quarter * 32 + lane, nw = n0 + chalf * WC;
+      // (rows and columns past the matrix multiply zeros; their scales are read inside it)
+      const float* sa = args.sa + min(m, args.M - 1);
+      const float* sw = args.sw + static_cast<size_t>(min(nw, args.N - 1) >> 7) * args.sw_n;
+      float acc_r[WC];
+#pragma unroll
+      for (int i = 0; i < WC; ++i) acc_r[i] = 0.f;
+      float s_next = __ldg(sa + static_cast<size_t>(k0) * args.M) * __ldg(sw + static_cast<size_t>(k0) * args.sw_k);
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int acc = it % NACC;
+        const float s = s_next;
+        const int kn = min(kb + 1, k1 - 1);
+        s_next = __ldg(sa + static_cast<size_t>(kn) * args.M) * __ldg(sw + static_cast<size_t>(kn) * args.sw_k);
+        if (!mbar_wait_warp(done_bar(stage), phase, wctx, 24)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t tb = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN + chalf * WC;
+#pragma unroll
+        for (int c4 = 0; c4 < WC / 32; ++c4) {
+          uint32_t r[32];
+          tc_ld32(tb + c4 * 32, r);
+          tc_wait_ld();
+          if (c4 == WC / 32 - 1) {     // the accumulator has been read: back to the matrix warp
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (CTAS == 1 || is_leader) mbar_arrive(free_bar(acc));
+              else mbar_arrive_cluster(mapa_u32(free_bar(acc), 0));
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc_r[c4 * 32 + j] = fmaf(s, __uint_as_float(r[j]), acc_r[c4 * 32 + j]);
+        }
+        if (++stage == NST) { stage = 0; phase ^= 1u; }
+      }
+      if (!ok) break;
+      if (args.split > 1) {
+        float* dst = args.parts + ((static_cast<size_t>(u) * CTAS + cta_rank) * 8 + ew) * (WC * 32);
+#pragma unroll
+        for (int c4 = 0; c4 < WC / 32; ++c4)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            reinterpret_cast<float4*>(dst + c4 * 1024)[j * 32 + lane] =
+                make_float4(acc_r[c4 * 32 + 4 * j], acc_r[c4 * 32 + 4 * j + 1], acc_r[c4 * 32 + 4 * j + 2], acc_r[c4 * 32 + 4 * j + 3]);
+        continue;
+      }
+      const int row0 = m0 + quarter * 32;
+      if (row0 >= args.M) continue;
+#pragma unroll
+      for (int c4 = 0; c4 < WC / 32; ++c4) {
+        const int n = nw + c4 * 32;
+        if (n >= args.N) break;
+        float* v = acc_r + c4 * 32;
+        if (args.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (n + j < args.N) v[j] += load_as(args.bias, args.bias_dt, n + j);
+        }
+        if (args.direct_out || args.out_dt == FDP_F32) {
+          box_wait(lane);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            box_put(box, lane, j, __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+          if (!args.direct_out) {
+            box_send(box, &tmOut, n, row0, lane);
+          } else {
+            __syncwarp();
+            const int rows = min(BOX_ROWS, args.M - row0);
+            const size_t at = static_cast<size_t>(row0) * args.N + n + lane;
+            const bool in = n + lane < args.N;
+            if (args.out_dt == FDP_F32) f8_store_rows(static_cast<float*>(args.out) + at, args.N, box, rows, lane, in);
+            else if (args.out_dt == FDP_BF16) f8_store_rows(static_cast<__nv_bfloat16*>(args.out) + at, args.N, box, rows, lane, in);
+            else f8_store_rows(static_cast<__half*>(args.out) + at, args.N, box, rows, lane, in);
+            __syncwarp();
+          }
+        } else {
+          // 16-bit: two chunks of 32 columns fill a box (a lone one is sent half full; the map's box is 64 wide, so it waits
+          // for its second half only where the matrix has one)
+          if ((c4 & 1) == 0) box_wait(lane);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 w = args.out_dt == FDP_BF16 ? pack16<__nv_bfloat16>(v + 8 * j) : pack16<__half>(v + 8 * j);
+            box_put(box, lane, 4 * (c4 & 1) + j, w.x, w.y, w.z, w.w);
+          }
+          if ((c4 & 1) == 1 || n + 32 >= args.N) box_send(box, &tmOut, n - 32 * (c4 & 1), row0, lane);
+        }
+      }
+    }
+  }
+  // ================= teardown =================
+  if (warp >= 2) box_drain(lane);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (CTAS == 2) cluster_sync_all();   // neither CTA leaves (or frees TMEM) while its peer may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::%2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS), "n"(CTAS) : "memory");
+  }
+}
+
+// the parts of a K split, added in order, with the bias
+template <int CTAS, int BN>
+__global__ void __launch_bounds__(256) fp8_join_kernel(const __grid_constant__ Fp8Args args) {
+  constexpr int WC = F8Tile<CTAS, BN>::WC, UNIT = CTAS * F8_BM * BN;
+  pdl_wait();
+  // a thread takes four columns of a row: rows of a box lie 16 bytes apart
+  const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int tile = static_cast<int>(i / (UNIT / 4)), e = static_cast<int>(i % (UNIT / 4)) * 4;
+  if (tile >= args.tiles_m * args.tiles_n) return;
+  const int wbox = e / 1024, in_box = e % 1024;
+  const int c4 = wbox % (WC / 32), cw = wbox / (WC / 32), ew = cw % 8, rank = cw / 8;
+  // epilogue warp ew is warp ew + 2 of its CTA: lane quarter (ew + 2) % 4, column half ew / 4
+  const int per_group = args.m_group * args.tiles_n;
+  const int g = tile / per_group, r = tile - g * per_group;
+  const int gm = min(args.m_group, args.tiles_m - g * args.m_group);
+  const int row = (g * args.m_group + r % gm) * (F8_BM * CTAS) + rank * F8_BM + ((ew + 2) & 3) * 32 + (in_box % 128) / 4;
+  const int n = r / gm * BN + (ew >> 2) * WC + c4 * 32 + in_box / 128 * 4;
+  if (row >= args.M || n >= args.N) return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < args.split; ++p) {
+    const float4 t = *reinterpret_cast<const float4*>(args.parts + (static_cast<size_t>(tile) * args.split + p) * UNIT + e);
+    v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+  }
+  for (int k = 0; k < 4 && n + k < args.N; ++k)
+    store_as(args.out, args.out_dt, static_cast<size_t>(row) * args.N + n + k, v[k] + (args.bias != nullptr ? load_as(args.bias, args.bias_dt, n + k) : 0.f));
+}
+
+bool make_bytes_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {pitch};
+  const cuuint32_t box[2] = {128, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int CTAS, int BN>
+int gemm_launch(const Fp8Args& args_in, const void* a, int pitch_a, const void* w, int pitch_w, int K, const Fp8Plan& pl, cudaStream_t s) {
+  static std::mutex mu;
+  static bool done[64];
+  if (!smem_opt_in(done, mu, fp8_gemm_kernel<CTAS, BN>, F8_SMEM)) return FDP_ERR_LAUNCH;
+  Fp8Args args = args_in;
+  args.tiles_m = ceil_div(args.M, F8_BM * CTAS);
+  args.tiles_n = ceil_div(args.N, BN);
+  args.split = pl.split;
+  args.m_group = args.tiles_m < 8 ? args.tiles_m : 8;
+  args.sticky = sticky_status_slot();
+  CUtensorMap ma, mb, mo;
+  if (!make_bytes_map(&ma, a, args.M, K, pitch_a, F8_BM) || !make_bytes_map(&mb, w, args.N, K, pitch_w, BN / CTAS)) return FDP_ERR_LAUNCH;
+  args.direct_out = static_cast<size_t>(args.N) * dtype_size(args.out_dt) % 16 != 0 || !aligned16(args.out);
+  if (args.direct_out || args.split > 1) mo = ma;
+  else if (!make_out_map(&mo, args.out, args.M, args.N, args.out_dt)) return FDP_ERR_LAUNCH;
+  const int units = args.tiles_m * args.tiles_n * args.split, workers = launch_sms() / CTAS;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(CTAS * (units < workers ? units : workers));
+  cfg.blockDim = dim3(F8_THREADS);
+  cfg.dynamicSmemBytes = F8_SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  if (CTAS == 2) {
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = 2; attr[na].val.clusterDim.y = 1; attr[na].val.clusterDim.z = 1;
+    ++na;
+  }
+  if (pdl_enabled()) {
+    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[na].val.programmaticStreamSerializationAllowed = 1;
+    ++na;
+  }
+  cfg.attrs = attr; cfg.numAttrs = na;
+  if (cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<CTAS, BN>, ma, mb, mo, args) != cudaSuccess) { cudaGetLastError(); return FDP_ERR_LAUNCH; }
+  note_launch();
+  if (args.split > 1) {
+    const size_t threads = static_cast<size_t>(args.tiles_m) * args.tiles_n * (CTAS * F8_BM * BN / 4);
+    launch_dependent(fp8_join_kernel<CTAS, BN>, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, args);
+    note_launch();
+  }
+  return FDP_OK;
+}
+
+template <typename T>
+void rows_typed(const void* x, uint8_t* q, float* scales, int rows, int cols, int pitch, cudaStream_t s) {
+  const int kblocks = ceil_div(cols, 128), row_tiles = ceil_div(rows, 16);
+  const unsigned grid = static_cast<unsigned>(row_tiles) * ceil_div(kblocks, QKB);
+  const T* xt = static_cast<const T*>(x);
+  if (cols % 8 == 0 && aligned16(x)) fp8_rows_kernel<T, true><<<grid, 256, 0, s>>>(xt, q, scales, rows, cols, pitch, kblocks, row_tiles);
+  else fp8_rows_kernel<T, false><<<grid, 256, 0, s>>>(xt, q, scales, rows, cols, pitch, kblocks, row_tiles);
+  note_launch();
+}
+template <typename T>
+void weight_typed(const void* w, uint8_t* q, uint8_t* qt, float* scales, int rows, int cols, int pitch, int pitch_t, cudaStream_t s) {
+  const int cb = ceil_div(cols, 128);
+  const unsigned grid = static_cast<unsigned>(ceil_div(rows, 128)) * cb;
+  const T* wt = static_cast<const T*>(w);
+  if (cols % 8 == 0 && aligned16(w)) fp8_weight_kernel<T, true><<<grid, 256, 0, s>>>(wt, q, qt, scales, rows, cols, pitch, pitch_t, cb);
+  else fp8_weight_kernel<T, false><<<grid, 256, 0, s>>>(wt, q, qt, scales, rows, cols, pitch, pitch_t, cb);
+  note_launch();
+}
+
+}  // namespace
+
+void fp8_rows(const void* x, void* q, float* scales, int rows, int cols, int pitch, int dt, cudaStream_t s) {
+  uint8_t* b = static_cast<uint8_t*>(q);
+  if (dt == FDP_F32) rows_typed<float>(x, b, scales, rows, cols, pitch, s);
+  else if (dt == FDP_BF16) rows_typed<__nv_bfloat16>(x, b, scales, rows, cols, pitch, s);
+  else rows_typed<__half>(x, b, scales, rows, cols, pitch, s);
+}
+void fp8_weight(const void* w, void* q, void* qt, float* scales, int rows, int cols, int pitch, int pitch_t, int dt, cudaStream_t s) {
+  uint8_t *b = static_cast<uint8_t*>(q), *bt = static_cast<uint8_t*>(qt);
+  if (dt == FDP_F32) weight_typed<float>(w, b, bt, scales, rows, cols, pitch, pitch_t, s);
+  else if (dt == FDP_BF16) weight_typed<__nv_bfloat16>(w, b, bt, scales, rows, cols, pitch, pitch_t, s);
+  else weight_typed<__half>(w, b, bt, scales, rows, cols, pitch, pitch_t, s);
+}
+
+Fp8Plan fp8_plan(int M, int N, int K) {
+  Fp8Plan pl;
+  const int kb = ceil_div(K, 128);
+  const long long pairs = static_cast<long long>(ceil_div(M, 256)) * ceil_div(N, 256);
+  // pair tiles where they fill the GPU, else single CTAs' tiles, cut along K where even those are few
+  if (pairs >= 74) { pl.ctas = 2; pl.bn = 256; pl.split = 1; }
+  else {
+    pl.ctas = 1; pl.bn = 128;
+    const long long tiles = static_cast<long long>(ceil_div(M, 128)) * ceil_div(N, 128);
+    long long split = 148 / tiles;
+    if (split > kb / 4) split = kb / 4;
+    pl.split = split < 1 ? 1 : static_cast<int>(split);
+  }
+  pl.parts_bytes = pl.split > 1 ? static_cast<size_t>(ceil_div(M, F8_BM * pl.ctas)) * ceil_div(N, pl.bn) * pl.split * pl.ctas * F8_BM * pl.bn * sizeof(float) : 0;
+  return pl;
+}
+
+int fp8_gemm(const void* a, int pitch_a, const float* sa, const void* w, int pitch_w, const float* sw, int sw_n, int sw_k, const void* bias,
+             int bias_dt, void* out, int M, int N, int K, int out_dt, float* parts, const Fp8Plan& pl, cudaStream_t s) {
+  Fp8Args args{};
+  args.M = M; args.N = N; args.kblocks = ceil_div(K, 128);
+  args.sa = sa; args.sw = sw; args.sw_n = sw_n; args.sw_k = sw_k;
+  args.out = out; args.out_dt = out_dt; args.bias = bias; args.bias_dt = bias_dt; args.parts = parts;
+  if (pl.ctas == 2) return gemm_launch<2, 256>(args, a, pitch_a, w, pitch_w, K, pl, s);
+  return gemm_launch<1, 128>(args, a, pitch_a, w, pitch_w, K, pl, s);
+}
+
+}  // namespace fdp

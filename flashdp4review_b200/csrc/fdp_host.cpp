@@ -41,6 +41,11 @@ struct Abi {
   decltype(&fdp_group_norm_fwd) group_norm_fwd;
   decltype(&fdp_group_norm_bwd_workspace_bytes) group_norm_bwd_workspace_bytes;
   decltype(&fdp_group_norm_bwd) group_norm_bwd;
+  decltype(&fdp_fp8_pitch) fp8_pitch;
+  decltype(&fdp_fp8_quantize) fp8_quantize;
+  decltype(&fdp_fp8_quantize_weight) fp8_quantize_weight;
+  decltype(&fdp_fp8_matmul_workspace_bytes) fp8_matmul_workspace_bytes;
+  decltype(&fdp_fp8_matmul) fp8_matmul;
 } abi;
 
 void bind(const std::map<std::string, uint64_t>& fns) {
@@ -53,6 +58,7 @@ void bind(const std::map<std::string, uint64_t>& fns) {
   FDP_BIND(dropout);
   FDP_BIND(group_norm_fwd_workspace_bytes); FDP_BIND(group_norm_fwd);
   FDP_BIND(group_norm_bwd_workspace_bytes); FDP_BIND(group_norm_bwd);
+  FDP_BIND(fp8_pitch); FDP_BIND(fp8_quantize); FDP_BIND(fp8_quantize_weight); FDP_BIND(fp8_matmul_workspace_bytes); FDP_BIND(fp8_matmul);
 #undef FDP_BIND
 }
 
@@ -389,6 +395,56 @@ py::tuple group_norm_bwd(const Tensor& dy, const Tensor& x, const OptTensor& w, 
   return py::make_tuple(st, dx, dgamma, dbeta, ng, nb);
 }
 
+// rows x pitch bytes, seen as rows x cols
+Tensor fp8_matrix(const Tensor& like, int64_t rows, int64_t cols) {
+  return new_tensor(like, {rows, abi.fp8_pitch(static_cast<int>(cols))}, at::kFloat8_e4m3fn).narrow(1, 0, cols);
+}
+// x [rows, cols] -> 8-bit numbers, scales [column blocks, rows]
+py::tuple fp8_quantize(const Tensor& x, int dt) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t rows = x.size(0), cols = x.size(1);
+  const Tensor q = fp8_matrix(x, rows, cols), scales = new_tensor(x, {(cols + 127) / 128, rows}, at::kFloat);
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = abi.fp8_quantize(ptr(x), ptr(q), static_cast<float*>(ptr(scales)), static_cast<int>(rows), static_cast<int>(cols), dt, stream(x));
+  }
+  return py::make_tuple(st, q, scales);
+}
+py::tuple fp8_quantize_weight(const Tensor& w, int dt) {
+  const c10::cuda::CUDAGuard guard(w.device());
+  const int64_t rows = w.size(0), cols = w.size(1);
+  const Tensor q = fp8_matrix(w, rows, cols), qt = fp8_matrix(w, cols, rows);
+  const Tensor scales = new_tensor(w, {(rows + 127) / 128, (cols + 127) / 128}, at::kFloat);
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = abi.fp8_quantize_weight(ptr(w), ptr(q), ptr(qt), static_cast<float*>(ptr(scales)), static_cast<int>(rows), static_cast<int>(cols), dt, stream(w));
+  }
+  return py::make_tuple(st, q, qt, scales);
+}
+// x (..., k) times w [n, k]^T in 8 bits
+py::tuple fp8_matmul(const Tensor& x, const Tensor& w, const Tensor& scales, const OptTensor& bias, int dt, int out_dt) {
+  const int64_t k = x.size(-1), n = w.size(0), rows = k > 0 ? x.numel() / k : 0;
+  if (w.device() != x.device() || scales.device() != x.device()) refuse("weight is on another device", w);
+  if (w.dim() != 2 || w.size(1) != k || w.scalar_type() != at::kFloat8_e4m3fn || w.stride(1) != 1 || w.stride(0) != abi.fp8_pitch(static_cast<int>(k)))
+    refuse("weight does not fit the other operand", w);
+  if (scales.scalar_type() != at::kFloat || scales.dim() != 2 || scales.size(0) != (n + 127) / 128 || scales.size(1) != (k + 127) / 128)
+    refuse("scales do not fit the weight", scales);
+  if (bias.has_value() && (bias->numel() != n || bias->device() != x.device() || bias->scalar_type() != x.scalar_type())) refuse("bias does not fit the output's columns", *bias);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor y = with_columns(x, n, out_dt);
+  const int r = static_cast<int>(rows), nn = static_cast<int>(n), kk = static_cast<int>(k);
+  const Tensor ws = workspace(x, abi.fp8_matmul_workspace_bytes(r, nn, kk));
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = abi.fp8_matmul(ptr(x), ptr(w), static_cast<const float*>(ptr(scales)), static_cast<int>(scales.stride(0)), static_cast<int>(scales.stride(1)),
+                        ptr(bias), ptr(y), r, nn, kk, dt, out_dt, ptr(ws), ws.numel(), stream(x));
+  }
+  return py::make_tuple(st, y);
+}
+
 // ---- the layers' autograd nodes --------------------------------------------------------------------------------------
 // What the Function classes of layers/*.py do, without a Python frame per tensor operation: a pass of a small layer is
 // bound by the host, and of its 120 to 160 us those classes took a third.  Choices and noise bookkeeping stay in
@@ -627,6 +683,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dropout", &dropout);
   m.def("group_norm_fwd", &group_norm_fwd);
   m.def("group_norm_bwd", &group_norm_bwd);
+  m.def("fp8_quantize", &fp8_quantize);
+  m.def("fp8_quantize_weight", &fp8_quantize_weight);
+  m.def("fp8_matmul", &fp8_matmul);
   m.def("bind_layers", &bind_layers);
   m.def("dp_linear", &dp_linear);
   m.def("dp_layernorm", &dp_layernorm);

@@ -124,6 +124,16 @@ int gn_fwd(const GnArgs& a, int dt, cudaStream_t s);
 // part: [2][B][chunks][C] (of dgamma, then of dbeta), what ln_psgrad_reduce takes; gpart: float2[B, chunks, G]
 int gn_bwd(const GnArgs& a, int dt, float* part, float* gpart, cudaStream_t s);
 
+// ---- e4m3 with a scale for each block of 128 (fdp_fp8.cu) ------------------------------------------------
+inline int fp8_pitch(int n) { return (n + 15) & ~15; }      // bytes of a row
+void fp8_rows(const void* x, void* q, float* scales, int rows, int cols, int pitch, int dt, cudaStream_t s);
+void fp8_weight(const void* w, void* q, void* qt, float* scales, int rows, int cols, int pitch, int pitch_t, int dt, cudaStream_t s);
+struct Fp8Plan { int ctas, bn, split; size_t parts_bytes; };
+Fp8Plan fp8_plan(int M, int N, int K);
+// out[M, N] = a[M, K] w[N, K]^T (+ bias), both in e4m3; follows the kernel that quantised `a` in the stream
+int fp8_gemm(const void* a, int pitch_a, const float* sa, const void* w, int pitch_w, const float* sw, int sw_n, int sw_k, const void* bias,
+             int bias_dt, void* out, int M, int N, int K, int out_dt, float* parts, const Fp8Plan& pl, cudaStream_t s);
+
 // ---- LayerNorm -----------------------------------------------------------------------------------
 struct LnPlan { int tpr, cpt, cw, rows_per_block, chunks; bool vec; };
 LnPlan ln_plan(int B, int T, int d, int dt);

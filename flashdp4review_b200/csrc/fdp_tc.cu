@@ -25,8 +25,70 @@
 #include "fdp_async.cuh"
 #include "fdp_gram_units.h"
 #include "fdp_kernels.h"
+#include "fdp_tcgen05.cuh"
 
 namespace fdp {
+
+EncodeTiledFn encode_fn() {
+  static std::mutex mu;
+  static EncodeTiledFn fn = nullptr;
+  std::lock_guard<std::mutex> lk(mu);
+  if (fn == nullptr) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+    else
+      cudaGetLastError();
+  }
+  return fn;
+}
+
+// Map of an output matrix [rows, cols] for the epilogue warps' boxes of 32 rows x 128 bytes.  The row pitch
+// has to be a multiple of 16 bytes and the base 16-byte aligned.
+bool make_out_map(CUtensorMap* m, void* base, uint64_t rows, uint64_t cols, int dt) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {cols * dtype_size(dt)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / dtype_size(dt)), BOX_ROWS};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(m, dt == FDP_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dt == FDP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
+// SMs of the current device (cached per device).
+static int sm_count() {
+  static std::mutex mu;
+  static int cache[64];
+  static bool have[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 148; }
+  std::lock_guard<std::mutex> lk(mu);
+  if (!have[dev]) {
+    int n = 148;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); n = 148; }
+    cache[dev] = n; have[dev] = true;
+  }
+  return cache[dev];
+}
+// SMs the next persistent GEMM grid may occupy: all of them minus the current reservation
+// (fdp_set_sm_reserve; FDP_TC_RESERVE_SMS is its initial value).  A persistent CTA holds a whole SM's
+// shared memory, so a collective kernel launched beside such a grid cannot start until SMs are free;
+// a caller that overlaps a GEMM with a collective reserves a few SMs for the duration of that call.
+static std::atomic<int> g_sm_reserve{[] { const char* e = getenv("FDP_TC_RESERVE_SMS"); return e ? atoi(e) : 0; }()};
+int launch_sms() {
+  int n = sm_count();
+  const int reserve = g_sm_reserve.load(std::memory_order_relaxed);
+  if (n > MAX_SMS) n = MAX_SMS;   // the parking area is sized for MAX_SMS workers
+  if (reserve > 0 && n - reserve >= 16) n -= reserve;
+  return n & ~1;  // CTA pairs
+}
+
 namespace {
 
 constexpr int BM = 128, BN = 256, BK = 64, STAGES = 4, UMMA_K = 16;
@@ -34,7 +96,6 @@ constexpr int A_STAGE_BYTES = BM * BK * 2;  // 16 KiB
 constexpr int B_STAGE_BYTES = BN * BK * 2;  // 32 KiB
 constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
 constexpr int BAR_BYTES = 256;
-constexpr int BOX_ROWS = 32, BOX_BYTES = BOX_ROWS * 128;   // an epilogue warp's output box: 32 rows of 128 bytes
 // EPI_STORE_SCALED keeps the clip factors of up to MAX_SMEM_FACTORS samples in shared memory (what the
 // ring and the output boxes leave of the 227 KB); larger batches read them from global memory
 constexpr int MAX_SMEM_FACTORS = 384;
@@ -43,12 +104,10 @@ constexpr int SMEM_BYTES_STORE = SMEM_BYTES + 8 * BOX_BYTES;
 constexpr int SMEM_BYTES_SCALED = SMEM_BYTES_STORE + MAX_SMEM_FACTORS * 4;
 static_assert(SPLIT_MAXIMA_BYTES % 256 == 0 && SPLIT_MAXIMA_BYTES >= (148 * 16 + 2) * sizeof(unsigned), "a word for every block of tc_split");
 static_assert(SMEM_BYTES_SCALED <= 227 * 1024, "shared memory of one CTA");
-constexpr int TMEM_COLS = 512;
 // Per-sample products kept in a call's workspace.  Beyond that there was nothing to gain: 4 x 2048 rows, 4096 -> 11008 bf16,
 // 721 MB of products, a layer's forward and backward 2148 us against 2157 (with the GEMMs before the uniform issue).
 constexpr size_t KEEP_LIMIT = static_cast<size_t>(512) << 20;
 constexpr int KEEP_SMEM_FACTORS = 128;
-constexpr int MAX_SMS = 148;           // workers the split-K parking area is sized for
 
 // EPI_STORE_SCALED: the accumulator of each sample (K segment) is drained on its own and added, times
 // that sample's clip factor, to fp32 registers of eight epilogue warps; G needs no scaled copy.
@@ -142,86 +201,6 @@ struct TcArgs {
   float* keep;          // chained EPI_*_SUMSQ (may be null): the product tiles, [tile][CTA of the pair][box]
 };
 
-// ---- PTX wrappers (mbarrier helpers live in fdp_async.cuh) --------------------------------------------
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
-}
-// ---- CTA-pair (cta_group::2) helpers: the even CTA of a 2-CTA cluster issues one 256-row MMA for both;
-// loads are per CTA (no multicast), completion is signalled on the leader's mbarrier ------------------
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// shared::cluster address of the same shared-memory offset in CTA `rank` of the cluster
-__device__ __forceinline__ uint32_t mapa_u32(uint32_t local_addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local_addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Hands an accumulator back to the leader's MMA warp.  Relaxed: no memory is handed over with it, the accumulator's loads
-// have completed (tcgen05.wait::ld), and tcgen05.fence::before_thread_sync here and ::after_thread_sync behind the MMA warp's
-// wait order them before its MMAs, for which the PTX manual's patterns between threads use a relaxed arrive and wait too.  A release at cluster scope waits for the warp's
-// own earlier stores and took 1300 to 2500 cycles, in which the pair's tensor cores ran dry (weight gradients in six products,
-// 16 x 197 rows 768 -> 3072: 151 us, now 134; 5 x 704, 64 -> 7928: 153 / 121; one pair alone in three products, 8192 deep: 89 / 64).
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t leader_bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(leader_bar) : "memory");
-}
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t leader_bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(leader_bar) : "memory");
-}
-// arrives on the barrier at this offset in both CTAs of the pair.  (One commit to both, not one each: a commit holds
-// the tensor pipe up by about 30 cycles; 32768 rows 4096 -> 4096 bf16: 732 -> 699 us.)
-__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-               ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t r[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// shared-memory matrix descriptor (sm_100 format): start address, leading / stride byte offsets in
-// 16-byte units, version 1, 128-byte swizzle.  The low word holds the address (and the leading offset), so that what
-// moves with the stage and the K slice is one 32-bit addition.
-struct Desc { uint32_t lo, hi; };
-__device__ __forceinline__ Desc make_desc(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
-  Desc d;
-  d.lo = ((saddr >> 4) & 0x3FFF) | (((lbo_bytes >> 4) & 0x3FFF) << 16);
-  d.hi = ((sbo_bytes >> 4) & 0x3FFF) | (1u << 14) /* descriptor version of sm_100 */ | (2u << 29) /* SWIZZLE_128B */;
-  return d;
-}
 // Descriptor of an operand whose first stage is at `saddr`, and the step of its low word to the k16-th UMMA_K slice.
 //  MN-major: 64-element (128 B) MN chunks of BK rows each, chunk stride BK*128 B (leading offset),
 //            8-row groups 1024 B apart (stride offset); a K=16 slice is 16 rows = 2048 B further.
@@ -241,17 +220,6 @@ __device__ __forceinline__ void tc_mma(uint32_t tmem_d, uint32_t a_lo, uint32_t 
       "tcgen05.mma.cta_group::%7.kind::f16 [%0], a, b, %5, p;\n\t}"
       ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "n"(CTAS) : "memory");
 }
-// one lane of the warp, the same one every time
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(p));
-  return p != 0;
-}
-
 // The Gaussian noise of 32 adjacent output elements starting at flat index idx0 (a multiple of 4: the
 // tensor-core kernels only see row pitches and column offsets that are multiples of 8).
 __device__ __forceinline__ void add_noise32(const NoiseKey& nk, size_t idx0, float v[32]) {
@@ -293,42 +261,6 @@ __device__ __forceinline__ void add_bias32(const TcArgs& args, int n, float v[32
   }
 }
 
-// ---- output boxes ------------------------------------------------------------------------------------
-// After tcgen05.ld a lane holds one row of the tile, so direct stores put the 32 lanes of an instruction
-// on 32 different rows: half-used sectors, 32 lines per request (16384 rows, 1024 -> 3072, bf16 forward with
-// bias: 171 us, tensor pipe 27 % busy; 86 us with the boxes and add_bias32).  Instead every epilogue warp
-// writes boxes of 32 rows x 128 bytes into its own 4 KB of shared memory, in the 128-byte swizzle of the
-// tensor map (16-byte chunk j of row r at slot j ^ (r & 7): no bank conflicts), and one lane hands each box
-// to the copy engine, which also clips what lies past the matrix.
-__device__ __forceinline__ void box_wait(int lane) {      // the previous box has been read out
-  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-  __syncwarp();
-}
-__device__ __forceinline__ void box_put(uint32_t box, int lane, int j, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-               ::"r"(box + lane * 128 + ((j ^ (lane & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-__device__ __forceinline__ void box_send(uint32_t box, const CUtensorMap* map, int col, int row, int lane) {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncwarp();
-  if (lane == 0) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(row), "r"(box) : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-  }
-}
-__device__ __forceinline__ void box_drain(int lane) {     // before the CTA leaves
-  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-}
-// 32 fp32 values per lane = one box
-__device__ __forceinline__ void store_f32x32(uint32_t box, const CUtensorMap* map, const float v[32], int col, int row, int lane) {
-  box_wait(lane);
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    box_put(box, lane, j, __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
-            __float_as_uint(v[4 * j + 3]));
-  box_send(box, map, col, row, lane);
-}
 // A kept product leaves straight from the registers, 32 x 32 elements at a time in the order that suits them: element
 // group j (four columns) of all 32 rows, then the next, so that every store of a warp is 512 contiguous bytes.  Through
 // shared memory and the copy engine, as an output goes, the stores compete with the operands for shared memory
@@ -1419,26 +1351,6 @@ __global__ void __launch_bounds__(256, 4) split_stats_kernel(const float* __rest
 }
 
 // ---- host side ------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static std::mutex mu;
-  static EncodeTiledFn fn = nullptr;
-  std::lock_guard<std::mutex> lk(mu);
-  if (fn == nullptr) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-    else
-      cudaGetLastError();
-  }
-  return fn;
-}
-
 // 2-D map over a row-major [rows, cols] matrix of 16-bit elements, 128-byte swizzle, zero fill
 // (rows of `pitch` elements, 0: as many as there are columns)
 bool make_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint32_t box_cols,
@@ -1486,22 +1398,6 @@ bool make_parts_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t co
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Map of an output matrix [rows, cols] for the epilogue warps' boxes of 32 rows x 128 bytes.  The row pitch
-// has to be a multiple of 16 bytes and the base 16-byte aligned.
-bool make_out_map(CUtensorMap* m, void* base, uint64_t rows, uint64_t cols, int dt) {
-  EncodeTiledFn fn = encode_fn();
-  if (fn == nullptr) return false;
-  const cuuint64_t dims[2] = {cols, rows};
-  const cuuint64_t strides[1] = {cols * dtype_size(dt)};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / dtype_size(dt)), BOX_ROWS};
-  const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = fn(m, dt == FDP_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dt == FDP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                        2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
-}
-
 uint32_t make_idesc(int dt, bool a_mn, bool b_mn, int ctas = 1, int n = BN) {
   uint32_t d = 0;
   d |= 1u << 4;                                   // accumulator format: F32
@@ -1512,34 +1408,6 @@ uint32_t make_idesc(int dt, bool a_mn, bool b_mn, int ctas = 1, int n = BN) {
   d |= static_cast<uint32_t>(n >> 3) << 17;       // N
   d |= static_cast<uint32_t>((BM * ctas) >> 4) << 24;  // M (256 for a CTA pair)
   return d;
-}
-
-// SMs of the current device (cached per device).
-int sm_count() {
-  static std::mutex mu;
-  static int cache[64];
-  static bool have[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 148; }
-  std::lock_guard<std::mutex> lk(mu);
-  if (!have[dev]) {
-    int n = 148;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); n = 148; }
-    cache[dev] = n; have[dev] = true;
-  }
-  return cache[dev];
-}
-// SMs the next persistent GEMM grid may occupy: all of them minus the current reservation
-// (fdp_set_sm_reserve; FDP_TC_RESERVE_SMS is its initial value).  A persistent CTA holds a whole SM's
-// shared memory, so a collective kernel launched beside such a grid cannot start until SMs are free;
-// a caller that overlaps a GEMM with a collective reserves a few SMs for the duration of that call.
-std::atomic<int> g_sm_reserve{[] { const char* e = getenv("FDP_TC_RESERVE_SMS"); return e ? atoi(e) : 0; }()};
-int launch_sms() {
-  int n = sm_count();
-  const int reserve = g_sm_reserve.load(std::memory_order_relaxed);
-  if (n > MAX_SMS) n = MAX_SMS;   // the parking area is sized for MAX_SMS workers
-  if (reserve > 0 && n - reserve >= 16) n -= reserve;
-  return n & ~1;  // CTA pairs
 }
 
 template <bool A_MN, bool B_MN, int EPI, int CTAS = 1>

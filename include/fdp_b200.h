@@ -34,7 +34,7 @@ extern "C" {
  *    accepted in the dtype of fdp_linear_dgrad / fdp_linear_fwd.
  * 4: FDP_FP32_WIDE, fdp_linear_bwd.
  * 5: FDP_KEEP_PRODUCTS, FDP_FP32_WIDE_GEMM, FDP_GEMM_SPLIT_K, FDP_PAD_16BIT.
- * 6: fdp_group_norm_fwd / _bwd, fdp_dropout. */
+ * 6: fdp_group_norm_fwd / _bwd, fdp_dropout, fdp_fp8_quantize / _weight, fdp_fp8_matmul. */
 #define FDP_ABI_VERSION 6
 
 typedef void* fdp_stream_t; /* a cudaStream_t */
@@ -348,6 +348,27 @@ int fdp_group_norm_bwd(const void* dy, const void* x, const void* gamma, const v
                        int B, int T, int C, int G, int activation, int dtype, int param_dtype,
                        const fdp_dropout_params* drop, const fdp_dp_params* p, void* workspace, size_t workspace_bytes,
                        fdp_stream_t stream);
+
+/* ---- products in 8-bit floating point with a scale for each block of 128 ------------------------------
+ * No counterpart in the reference.  Numbers are held in e4m3 (no infinities, largest 448) with one scale for each block: a
+ * power of two, the smallest that brings the block's largest finite magnitude to at most 448 (1 for a block of zeros; at least 2^-126).
+ * A number that is not finite is held as a NaN.  Rows of 8-bit numbers have a pitch of fdp_fp8_pitch(columns) bytes.
+ * fdp_fp8_quantize: activations and gradients, blocks of 1 x 128, so that no scale mixes rows (samples).
+ *   x [rows,cols] in `dtype` -> q [rows, pitch(cols)] bytes, scales float[ceil(cols / 128)][rows].
+ * fdp_fp8_quantize_weight: blocks of 128 x 128, as it lies and transposed (each product contracts over adjacent bytes).
+ *   w [rows,cols] -> q [rows, pitch(cols)], qt [cols, pitch(rows)], scales float[ceil(rows / 128)][ceil(cols / 128)].
+ * fdp_fp8_matmul: y[rows,n] = quantised(x[rows,k]) * w[n,k]^T (+ bias[n]), accumulated in fp32, rounded once; x and bias in
+ *   `dtype`, y in `out_dtype`, w [n, pitch(k)] bytes whose scale of block (i, j) (128 rows i, 128 columns j) is
+ *   w_scales[i * scale_stride_n + j * scale_stride_k].  The forward product of a layer is this with its weight [out,in],
+ *   its input gradient with the weight transposed.  w 16-byte aligned.
+ */
+int fdp_fp8_pitch(int cols);
+int fdp_fp8_quantize(const void* x, void* q, float* scales, int rows, int cols, int dtype, fdp_stream_t stream);
+int fdp_fp8_quantize_weight(const void* w, void* q, void* qt, float* scales, int rows, int cols, int dtype, fdp_stream_t stream);
+size_t fdp_fp8_matmul_workspace_bytes(int rows, int n, int k);
+int fdp_fp8_matmul(const void* x, const void* w, const float* w_scales, int scale_stride_n, int scale_stride_k,
+                   const void* bias, void* y, int rows, int n, int k, int dtype, int out_dtype, void* workspace,
+                   size_t workspace_bytes, fdp_stream_t stream);
 
 #ifdef __cplusplus
 }

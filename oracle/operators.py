@@ -80,3 +80,27 @@ def clipped_mean(per_sample, C, clamp, divisor=None):
     norms = per_sample.square().sum(1).sqrt()
     f = torch.from_numpy(O.clip_factor(norms.numpy(), C, clamp))
     return (per_sample * f[:, None]).sum(0) / (divisor or per_sample.shape[0]), norms
+
+
+def e4m3_blocks(a, down):
+    """(the numbers, the scales) that `a` [r, c] stands for in e4m3 with one power-of-two scale for each block of down x 128:
+    values float64 (before the scale), scales float64 [ceil(r / down), ceil(c / 128)]."""
+    a = a.detach().cpu().double()
+    r, c = a.shape
+    rb, cb = -(-r // down), -(-c // 128)
+    mag = torch.where(torch.isfinite(a), a.abs(), 0.0)
+    padded = torch.zeros(rb * down, cb * 128, dtype=torch.float64)
+    padded[:r, :c] = mag
+    top = padded.view(rb, down, cb, 128).amax((1, 3))
+    m, e = torch.frexp(top)
+    k = torch.where(top > 0, (e - torch.where(m <= 0.875, 9, 8)).clamp(min=-126), torch.zeros_like(e))
+    scale = torch.ldexp(torch.ones_like(top), k)
+    v = a / scale.repeat_interleave(down, 0)[:r].repeat_interleave(128, 1)[:, :c]
+    # three bits behind the leading one, which does not go below 2^-6; round to nearest even
+    step = torch.ldexp(torch.ones_like(v), (torch.frexp(v)[1] - 1).clamp(min=-6) - 3)
+    return torch.where(torch.isfinite(a), torch.round(v / step) * step, math.nan), scale
+
+
+def e4m3_stands_for(a, down):
+    v, s = e4m3_blocks(a, down)
+    return v * s.repeat_interleave(down, 0)[: a.shape[0]].repeat_interleave(128, 1)[:, : a.shape[1]]
