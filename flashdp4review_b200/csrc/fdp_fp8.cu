@@ -215,6 +215,42 @@ __host__ __device__ constexpr uint32_t f8_idesc(int ctas, int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>((F8_BM * ctas) >> 4) << 24);
 }
 
+// acc += s * v for two adjacent numbers in one instruction
+__device__ __forceinline__ void fma2(float2& acc, uint32_t v0, uint32_t v1, float s) {
+  asm("{\n\t.reg .b64 a, b, c;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %4};\n\t"
+      "mov.b64 c, {%0, %1};\n\t"
+      "fma.rn.f32x2 c, a, b, c;\n\t"
+      "mov.b64 {%0, %1}, c;\n\t}"
+      : "+f"(acc.x), "+f"(acc.y) : "r"(v0), "r"(v1), "f"(s));
+}
+// v[0..31] += bias[n..n+31], the same numbers in every lane: 16-byte loads where they may be
+__device__ __forceinline__ void f8_add_bias(const void* bias, int dt, int n, int N, float v[32]) {
+  if (n + 32 <= N && (reinterpret_cast<uintptr_t>(bias) & 15) == 0) {
+    if (dt == FDP_F32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(bias) + n) + j);
+        v[4 * j] += b.x; v[4 * j + 1] += b.y; v[4 * j + 2] += b.z; v[4 * j + 3] += b.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(bias) + n) + j);
+        float b[8];
+        if (dt == FDP_BF16) unpack16<__nv_bfloat16>(raw, b); else unpack16<__half>(raw, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * j + e] += b[e];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (n + j < N) v[j] += load_as(bias, dt, n + j);
+  }
+}
+
 // rows of a warp's box one by one: an output that the copy engine cannot write
 template <typename T>
 __device__ __forceinline__ void f8_store_rows(T* out, size_t ld, uint32_t box, int rows, int lane, bool in) {
@@ -371,9 +407,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       // (rows and columns past the matrix multiply zeros; their scales are read inside it)
       const float* sa = args.sa + min(m, args.M - 1);
       const float* sw = args.sw + static_cast<size_t>(min(nw, args.N - 1) >> 7) * args.sw_n;
-      float acc_r[WC];
+      float2 acc2[WC / 2];
 #pragma unroll
-      for (int i = 0; i < WC; ++i) acc_r[i] = 0.f;
+      for (int i = 0; i < WC / 2; ++i) acc2[i] = make_float2(0.f, 0.f);
       float s_next = __ldg(sa + static_cast<size_t>(k0) * args.M) * __ldg(sw + static_cast<size_t>(k0) * args.sw_k);
       for (int kb = k0; kb < k1; ++kb, ++it) {
         const int acc = it % NACC;
@@ -383,12 +419,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         if (!mbar_wait_warp(done_bar(stage), phase, wctx, 24)) { ok = false; break; }
         tc_fence_after();
         const uint32_t tb = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN + chalf * WC;
+        // a chunk of 32 columns is on its way while the one before it is added
+        uint32_t r[2][32];
+        tc_ld32(tb, r[0]);
+        tc_wait_ld();
 #pragma unroll
         for (int c4 = 0; c4 < WC / 32; ++c4) {
-          uint32_t r[32];
-          tc_ld32(tb + c4 * 32, r);
-          tc_wait_ld();
-          if (c4 == WC / 32 - 1) {     // the accumulator has been read: back to the matrix warp
+          if (c4 + 1 < WC / 32) tc_ld32(tb + (c4 + 1) * 32, r[(c4 + 1) & 1]);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) fma2(acc2[c4 * 16 + j], r[c4 & 1][2 * j], r[c4 & 1][2 * j + 1], s);
+          if (c4 + 1 < WC / 32) tc_wait_ld();
+          if (c4 + 2 == WC / 32 || WC == 32) {     // the accumulator has been read: back to the matrix warp
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -396,12 +437,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
               else mbar_arrive_cluster(mapa_u32(free_bar(acc), 0));
             }
           }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc_r[c4 * 32 + j] = fmaf(s, __uint_as_float(r[j]), acc_r[c4 * 32 + j]);
         }
         if (++stage == NST) { stage = 0; phase ^= 1u; }
       }
       if (!ok) break;
+      float acc_r[WC];
+#pragma unroll
+      for (int i = 0; i < WC / 2; ++i) { acc_r[2 * i] = acc2[i].x; acc_r[2 * i + 1] = acc2[i].y; }
       if (args.split > 1) {
         float* dst = args.parts + ((static_cast<size_t>(u) * CTAS + cta_rank) * 8 + ew) * (WC * 32);
 #pragma unroll
@@ -419,11 +461,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         const int n = nw + c4 * 32;
         if (n >= args.N) break;
         float* v = acc_r + c4 * 32;
-        if (args.bias != nullptr) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (n + j < args.N) v[j] += load_as(args.bias, args.bias_dt, n + j);
-        }
+        if (args.bias != nullptr) f8_add_bias(args.bias, args.bias_dt, n, args.N, v);
         if (args.direct_out || args.out_dt == FDP_F32) {
           box_wait(lane);
 #pragma unroll
