@@ -130,16 +130,27 @@ Fp8Ws fp8_ws(void* base, int rows, int n, int k) {
   w.bytes = c.off;
   return w;
 }
-// workspace of fdp_group_norm_bwd
-struct GnBwdWs { float *sumsq, *factors, *gpart, *part; size_t bytes; };
-GnBwdWs gn_bwd_ws(void* base, int B, int T, int C, int G) {
-  GnBwdWs w;
-  const size_t chunks = gn_plan(B, T, C).chunks;
+// workspace of fdp_group_norm_fwd / _bwd.  The query knows neither dtype nor dropout: the largest of their plans.
+struct GnWs { float *gpart, *gsum, *part, *psgrad, *sumsq, *factors; size_t bytes; };
+GnWs gn_ws(void* base, int B, int T, int C, int G, bool backward) {
+  GnWs w{};
+  size_t chunks = 0, parts = 0;
+  for (const int element : {2, 4})
+    for (const bool drop : {false, true}) {
+      const GnPlan pl = gn_plan(B, T, C, G, element, backward ? 2 : 1, drop);
+      const size_t q = gn_sumsq_parts(C, pl);
+      if (static_cast<size_t>(pl.chunks) > chunks) chunks = pl.chunks;
+      if (q > parts) parts = q;
+    }
   Carver c(base);
-  w.sumsq = c.take<float>(static_cast<size_t>(2) * B * ln_sumsq_parts(C));
-  w.factors = c.take<float>(static_cast<size_t>(2) * B);
   w.gpart = c.take<float>(2 * B * chunks * G);
-  w.part = c.take<float>(2 * B * chunks * C);
+  w.gsum = c.take<float>(static_cast<size_t>(2) * B * G);
+  if (backward) {
+    w.part = c.take<float>(2 * B * chunks * C);
+    w.psgrad = c.take<float>(static_cast<size_t>(2) * B * C);
+    w.sumsq = c.take<float>(static_cast<size_t>(2) * B * parts);
+    w.factors = c.take<float>(static_cast<size_t>(2) * B);
+  }
   w.bytes = c.off;
   return w;
 }
@@ -853,7 +864,7 @@ int fdp_dropout(const void* x, const void* residual, void* y, size_t n, int dtyp
 
 size_t fdp_group_norm_fwd_workspace_bytes(int B, int T, int C, int G) {
   if (B <= 0 || T <= 0 || C <= 0 || G <= 0) return 0;
-  return sizeof(float) * 2 * B * static_cast<size_t>(gn_plan(B, T, C).chunks) * G;
+  return gn_ws(nullptr, B, T, C, G, false).bytes;
 }
 
 int fdp_group_norm_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd, int B, int T, int C, int G,
@@ -865,9 +876,11 @@ int fdp_group_norm_fwd(const void* x, const void* gamma, const void* beta, void*
   if (st != FDP_OK) return st;
   if ((st = current_device_ok()) != FDP_OK) return st;
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < fdp_group_norm_fwd_workspace_bytes(B, T, C, G)) return FDP_ERR_WORKSPACE;
+  const GnWs w = gn_ws(workspace, B, T, C, G, false);
   GnArgs a{};
   a.x = x; a.gamma = gamma; a.beta = beta; a.y = y; a.mean = mean; a.rstd = rstd;
-  a.B = B; a.T = T; a.C = C; a.G = G; a.act = activation; a.pdt = param_dtype; a.eps = eps; a.drop = drop; a.workspace = workspace;
+  a.B = B; a.T = T; a.C = C; a.G = G; a.act = activation; a.pdt = param_dtype; a.eps = eps; a.drop = drop;
+  a.gpart = w.gpart; a.gsum = w.gsum;
   if ((st = gn_fwd(a, dtype, static_cast<cudaStream_t>(stream))) != FDP_OK) return st;
   FDP_LAUNCH_OK();
   return FDP_OK;
@@ -875,7 +888,7 @@ int fdp_group_norm_fwd(const void* x, const void* gamma, const void* beta, void*
 
 size_t fdp_group_norm_bwd_workspace_bytes(int B, int T, int C, int G) {
   if (B <= 0 || T <= 0 || C <= 0 || G <= 0) return 0;
-  return gn_bwd_ws(nullptr, B, T, C, G).bytes;
+  return gn_ws(nullptr, B, T, C, G, true).bytes;
 }
 
 int fdp_group_norm_bwd(const void* dy, const void* x, const void* gamma, const void* beta, const float* mean, const float* rstd, void* dx,
@@ -891,20 +904,15 @@ int fdp_group_norm_bwd(const void* dy, const void* x, const void* gamma, const v
   if ((st = check_params(p)) != FDP_OK) return st;
   if ((st = current_device_ok()) != FDP_OK) return st;
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < fdp_group_norm_bwd_workspace_bytes(B, T, C, G)) return FDP_ERR_WORKSPACE;
-  const GnBwdWs w = gn_bwd_ws(workspace, B, T, C, G);
-  const int chunks = gn_plan(B, T, C).chunks;
+  const GnWs w = gn_ws(workspace, B, T, C, G, true);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   GnArgs a{};
   a.x = x; a.dy = dy; a.gamma = gamma; a.beta = beta; a.dx = dx;
   a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
   a.B = B; a.T = T; a.C = C; a.G = G; a.act = activation; a.pdt = param_dtype; a.drop = drop;
-  if ((st = gn_bwd(a, dtype, w.part, w.gpart, s)) != FDP_OK) return st;
-  if (dgamma != nullptr) {
-    const int div = p->batch_divisor > 0 ? p->batch_divisor : B;
-    ln_psgrad_reduce(w.part, w.sumsq, B, chunks, C, s);
-    ln_clip_finalize(w.part, w.sumsq, ln_sumsq_parts(C), p->C, p->clamp_value, w.factors, norms_gamma, norms_beta, dgamma, dbeta, B, chunks, C,
-                     param_dtype, 1.0f / static_cast<float>(div), make_noise_key(p, p->param_id), make_noise_key(p, p->param_id2), s);
-  }
+  a.gpart = w.gpart; a.gsum = w.gsum; a.part = w.part; a.psgrad = w.psgrad; a.sumsq = w.sumsq;
+  a.factors = w.factors;
+  if ((st = gn_bwd(a, dtype, p, dgamma, dbeta, norms_gamma, norms_beta, s)) != FDP_OK) return st;
   FDP_LAUNCH_OK();
   return FDP_OK;
 }

@@ -5,9 +5,18 @@
 //   dx = rstd * (gamma * gz - s1 - xhat * s2), s1 = sum_{c in g} gamma dbeta_b / n, s2 = sum_{c in g} gamma dgamma_b / n, n = T * C/G
 //
 // The per-channel sums that the group sums are made of are the per-sample parameter gradients that get clipped, so one
-// pass over (dy, x) serves both.  HBM-bound: a first kernel reduces, a second one reads the same data again (out of
-// L2 where the tensors fit it) and writes.  A row is C contiguous numbers; a thread keeps one column of eight channels and
-// walks rows, so that channel sums and parameters stay in registers.  All reductions run in a fixed order.
+// pass over (dy, x) serves both.
+//
+// Each direction reads its inputs twice, reductions first, then the result; the second pass runs from the back, so that what
+// the first one read last is still in L2.  A row is C contiguous numbers; a thread keeps one column (16 bytes) of channels
+// and walks rows, so that channel sums and parameters stay in registers.  All sums run in a fixed order.  What bounds it is
+// instruction issue as much as memory: at the memory's speed a 16-bit element leaves 22 issue slots a read and write, the
+// passes with an activation take 9 to 22, and what a block does beside its rows is worth six rows a thread more.
+// (Tried: one kernel a direction whose blocks draw reductions and results from a counter, so that nothing drains between the
+// passes.  A block that drew a result waited for reductions still running beside it: 16 x 4096 x 320 bf16 144 us for both
+// directions against 117 then with a kernel a pass.  Tried: sets of samples whose second pass finds all of them in L2:
+// 8 x 16384 x 256 fp32 217 us in sets of 100 MB, 292 of 48 MB, 199 without sets; each pass more costs more than its DRAM reads save.)
+#include "fdp_async.cuh"
 #include "fdp_dropout.cuh"
 #include "fdp_kernels.h"
 #include "fdp_vec8.cuh"
@@ -15,474 +24,1091 @@
 namespace fdp {
 namespace {
 
-constexpr int GN_THREADS = 256;
+constexpr int GN_THREADS = 256, GN_WARPS = GN_THREADS / 32;
+// blocks an SM holds, by their registers: with the generator's words and keys beside the numbers only two
+constexpr int gn_per_sm(bool drop) { return drop ? 2 : 3; }
 
-// V adjacent elements (V = 8 as 16-byte vectors, else one)
+// ---- V numbers of a thread --------------------------------------------------------------------------
+// As pairs of fp32 in 64-bit registers, on which one instruction does two operations (rounded as single ones are); V = 1 is a
+// plain float.  The pairs stay pairs: taken apart and put together again around every operation they cost more
+// instructions than they save.
+using pair_t = unsigned long long;
+__device__ __forceinline__ pair_t pair_of(float lo, float hi) {
+  pair_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void pair_get(pair_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ pair_t pair_add(pair_t a, pair_t b) { pair_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ pair_t pair_mul(pair_t a, pair_t b) { pair_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ pair_t pair_fma(pair_t a, pair_t b, pair_t c) {
+  pair_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+template <int V> struct Nums { pair_t p[V / 2]; };
+template <> struct Nums<1> { float x; };
+template <int V> __device__ __forceinline__ Nums<V> n_all(float v) {
+  Nums<V> r;
+  if constexpr (V == 1) { r.x = v; } else {
+    const pair_t q = pair_of(v, v);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.p[i] = q;
+  }
+  return r;
+}
+template <int V> __device__ __forceinline__ Nums<V> operator+(const Nums<V>& a, const Nums<V>& b) {
+  Nums<V> r;
+  if constexpr (V == 1) { r.x = a.x + b.x; } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.p[i] = pair_add(a.p[i], b.p[i]);
+  }
+  return r;
+}
+template <int V> __device__ __forceinline__ Nums<V> operator*(const Nums<V>& a, const Nums<V>& b) {
+  Nums<V> r;
+  if constexpr (V == 1) { r.x = a.x * b.x; } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.p[i] = pair_mul(a.p[i], b.p[i]);
+  }
+  return r;
+}
+template <int V> __device__ __forceinline__ Nums<V> n_fma(const Nums<V>& a, const Nums<V>& b, const Nums<V>& c) {
+  Nums<V> r;
+  if constexpr (V == 1) { r.x = fmaf(a.x, b.x, c.x); } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.p[i] = pair_fma(a.p[i], b.p[i], c.p[i]);
+  }
+  return r;
+}
+template <int V> __device__ __forceinline__ Nums<V> operator*(const Nums<V>& a, float s) { return a * n_all<V>(s); }
+template <int V> __device__ __forceinline__ void n_get(const Nums<V>& a, float f[V]) {
+  if constexpr (V == 1) { f[0] = a.x; } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) pair_get(a.p[i], f[2 * i], f[2 * i + 1]);
+  }
+}
+template <int V> __device__ __forceinline__ Nums<V> n_of(const float f[V]) {
+  Nums<V> r;
+  if constexpr (V == 1) { r.x = f[0]; } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.p[i] = pair_of(f[2 * i], f[2 * i + 1]);
+  }
+  return r;
+}
+
+// V adjacent elements of a tensor: one vector of 16 bytes (8 of 16 bits, 4 of 32), or of 4 bytes (2 of 16 bits: rows whose length
+// is only even), or one
+template <typename T, int V> struct Raw { uint4 w; };
+template <typename T> struct Raw<T, 2> { uint32_t w; };
 template <typename T, int V>
-__device__ __forceinline__ void load_v(const T* p, float f[V]) {
-  if constexpr (V == 8) unpack8(load8(p), f);
-  else f[0] = to_f32<T>(*p);
+__device__ __forceinline__ Nums<V> unpack_v(const Raw<T, V>& r) {
+  float g[8];
+  if constexpr (V == 2) unpack16<T>(make_uint4(r.w, 0, 0, 0), g);
+  else unpack16<T>(r.w, g);
+  return n_of<V>(g);
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_v(T* p, const float f[V]) {
-  if constexpr (V == 8) store8(p, f);
-  else *p = from_f32<T>(f[0]);
+__device__ __forceinline__ Nums<V> load_v(const T* p) {
+  if constexpr (V == 1) return Nums<1>{to_f32<T>(*p)};
+  else return unpack_v<T, V>(*reinterpret_cast<const Raw<T, V>*>(p));
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T* p, const Nums<V>& a) {
+  float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  n_get<V>(a, f);
+  if constexpr (V == 1) *p = from_f32<T>(f[0]);
+  else if constexpr (V == 2) *reinterpret_cast<uint32_t*>(p) = pack16<T>(f).x;
+  else *reinterpret_cast<uint4*>(p) = pack16<T>(f);
 }
 template <int V>
-__device__ __forceinline__ uint32_t keep_v(const DropKey& k, uint32_t step, size_t element) {
-  if constexpr (V == 8) return keep8(k, step, element >> 3);
-  else return keep1(k, step, element) ? 1u : 0u;
+__device__ __forceinline__ Nums<V> n_drop(const DropKey& k, uint32_t step, uint64_t element, const Nums<V>& a) {
+  float f[V];
+  n_get<V>(a, f);
+  drop_v<V>(k, step, element, f);
+  return n_of<V>(f);
 }
 
 // ---- activations -----------------------------------------------------------------------------------
-// exp for 16-bit tensors: two instructions, relative error 2^-22 for the arguments that matter, far below their rounding
-template <bool FAST> __device__ __forceinline__ float act_exp(float v) { return FAST ? __expf(v) : expf(v); }
-template <bool FAST> __device__ __forceinline__ float act_sigmoid(float v) {
-  const float d = 1.f + act_exp<FAST>(-v);
-  return FAST ? __fdividef(1.f, d) : 1.f / d;
+// ex2.approx is off by 2^-22 of its result and rcp.approx by 2^-23, and rounding v log2(e) adds |v| 2^-23; where |v| is large
+// enough for that to matter the result it is relative to has become small against z, so the error of an activation stays
+// at a few 2^-23 of z.
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
-constexpr float SQRT_2_PI = 0.7978845608028654f, INV_SQRT_2PI = 0.3989422804014327f, SQRT_HALF = 0.7071067811865476f;
-// gelu_tanh: (1 + tanh u) / 2 = sigmoid(2 u), which loses nothing where tanh u is near -1
-template <bool FAST> __device__ __forceinline__ float gelu_half(float z) {
-  return act_sigmoid<FAST>(2.f * SQRT_2_PI * z * fmaf(0.044715f * z, z, 1.f));
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
-// act(z) of V values
-template <bool FAST, int V>
-__device__ __forceinline__ void activate(int act, const float z[V], float a[V]) {
-  switch (act) {
-    case FDP_ACT_RELU:
+constexpr float LOG2E = 1.4426950408889634f, SQRT_2_PI = 0.7978845608028654f, INV_SQRT_2PI = 0.3989422804014327f, SQRT_HALF = 0.7071067811865476f;
+// 1 / (1 + 2^u).  Two reciprocals come from one, 1 / a = b / (a b): the special-function units, a quarter of an issue slot
+// wide, would otherwise be what bounds the passes (21 M elements x 2 of them: 9.4 us, 7 so).  u is held to 60, where the result is
+// 2^-60, so that a product of two is finite, also where one is a NaN (whose activation is one all the same, being a multiple of z).
+template <int V> __device__ __forceinline__ Nums<V> n_sigmoid2(const Nums<V>& u) {
+  float a[V];
+  n_get<V>(u, a);
 #pragma unroll
-      for (int e = 0; e < V; ++e) a[e] = z[e] > 0.f || isnan(z[e]) ? z[e] : 0.f;
-      break;
-    case FDP_ACT_SILU:
+  for (int e = 0; e < V; ++e) a[e] = ex2(fminf(a[e], 60.f));
+  if constexpr (V == 1) {
+    return Nums<1>{rcp(1.f + a[0])};
+  } else {
+    Nums<V> s;
+    const pair_t one = pair_of(1.f, 1.f);
 #pragma unroll
-      for (int e = 0; e < V; ++e) a[e] = z[e] * act_sigmoid<FAST>(z[e]);
-      break;
-    case FDP_ACT_GELU:
-#pragma unroll
-      for (int e = 0; e < V; ++e) a[e] = z[e] * fmaf(0.5f, erff(z[e] * SQRT_HALF), 0.5f);
-      break;
-    case FDP_ACT_GELU_TANH:
-#pragma unroll
-      for (int e = 0; e < V; ++e) a[e] = z[e] * gelu_half<FAST>(z[e]);
-      break;
-    default:
-#pragma unroll
-      for (int e = 0; e < V; ++e) a[e] = z[e];
+    for (int i = 0; i < V / 2; ++i) {
+      float x, y;
+      pair_get(pair_add(pair_of(a[2 * i], a[2 * i + 1]), one), x, y);
+      const float r = rcp(x * y);
+      s.p[i] = pair_of(y * r, x * r);
+    }
+    return s;
   }
 }
-// g[e] *= act'(z[e])
-template <bool FAST, int V>
-__device__ __forceinline__ void times_slope(int act, const float z[V], float g[V]) {
+// gelu_tanh: (1 + tanh w) / 2 = 1 / (1 + e^(-2 w)), which loses nothing where tanh w is near -1; w = sqrt(2/pi) (z + 0.044715 z^3)
+template <int V> __device__ __forceinline__ Nums<V> n_gelu_half(const Nums<V>& z) {
+  constexpr float K = -2.f * SQRT_2_PI * LOG2E;
+  return n_sigmoid2<V>(n_fma<V>(z * z, n_all<V>(K * 0.044715f), n_all<V>(K)) * z);
+}
+// act(z)
+template <int V>
+__device__ __forceinline__ Nums<V> activate(int act, const Nums<V>& z) {
   switch (act) {
-    case FDP_ACT_RELU:
+    case FDP_ACT_RELU: {
+      float f[V];
+      n_get<V>(z, f);
 #pragma unroll
-      for (int e = 0; e < V; ++e) g[e] = z[e] > 0.f ? g[e] : 0.f;
-      break;
+      for (int e = 0; e < V; ++e) f[e] = f[e] > 0.f || isnan(f[e]) ? f[e] : 0.f;
+      return n_of<V>(f);
+    }
     case FDP_ACT_SILU:
+      return n_sigmoid2<V>(z * -LOG2E) * z;
+    case FDP_ACT_GELU: {
+      float f[V];
+      n_get<V>(z, f);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float s = act_sigmoid<FAST>(z[e]);
-        g[e] *= s * fmaf(z[e], 1.f - s, 1.f);
-      }
-      break;
-    case FDP_ACT_GELU:
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        g[e] *= fmaf(z[e] * INV_SQRT_2PI, act_exp<FAST>(-0.5f * z[e] * z[e]), fmaf(0.5f, erff(z[e] * SQRT_HALF), 0.5f));
-      break;
+      for (int e = 0; e < V; ++e) f[e] *= fmaf(0.5f, erff(f[e] * SQRT_HALF), 0.5f);
+      return n_of<V>(f);
+    }
     case FDP_ACT_GELU_TANH:
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float h = gelu_half<FAST>(z[e]);
-        g[e] *= fmaf(z[e] * (h * (1.f - h)), 2.f * SQRT_2_PI * fmaf(3.f * 0.044715f * z[e], z[e], 1.f), h);
-      }
-      break;
+      return n_gelu_half<V>(z) * z;
     default:
-      break;
+      return z;
+  }
+}
+// g * act'(z)
+template <int V>
+__device__ __forceinline__ Nums<V> times_slope(int act, const Nums<V>& z, const Nums<V>& g) {
+  switch (act) {
+    case FDP_ACT_RELU: {
+      float f[V], h[V];
+      n_get<V>(z, f);
+      n_get<V>(g, h);
+#pragma unroll
+      for (int e = 0; e < V; ++e) h[e] = f[e] > 0.f ? h[e] : 0.f;
+      return n_of<V>(h);
+    }
+    case FDP_ACT_SILU: {                  // s (1 + z (1 - s)) = s + z s (1 - s)
+      const Nums<V> s = n_sigmoid2<V>(z * -LOG2E);
+      return g * n_fma<V>(n_fma<V>(s, n_all<V>(-1.f), n_all<V>(1.f)) * z, s, s);
+    }
+    case FDP_ACT_GELU: {
+      float f[V];
+      n_get<V>(z, f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = fmaf(f[e] * INV_SQRT_2PI, ex2(-0.5f * LOG2E * f[e] * f[e]), fmaf(0.5f, erff(f[e] * SQRT_HALF), 0.5f));
+      return g * n_of<V>(f);
+    }
+    case FDP_ACT_GELU_TANH: {             // h + z h (1 - h) 2 sqrt(2/pi) (1 + 3 * 0.044715 z^2)
+      constexpr float K = 2.f * SQRT_2_PI;
+      const Nums<V> h = n_gelu_half<V>(z);
+      const Nums<V> t = n_fma<V>(z * z, n_all<V>(K * 3.f * 0.044715f), n_all<V>(K)) * z;
+      return g * n_fma<V>(t, n_fma<V>(h, n_all<V>(-1.f), n_all<V>(1.f)) * h, h);
+    }
+    default:
+      return g;
   }
 }
 
-// ---- a block's share: rows [r0, r1) of sample b ------------------------------------------------------
-struct Span { int b, chunk, r0, r1; };
-__device__ __forceinline__ Span span_of(int chunks, int rows_per_chunk, int T) {
-  Span s;
-  s.b = blockIdx.x / chunks;
-  s.chunk = blockIdx.x - s.b * chunks;
-  s.r0 = s.chunk * rows_per_chunk;
-  s.r1 = min(T, s.r0 + rows_per_chunk);
+// ---- a block's share: rows [r0, r1) and channels [c0, c0 + C) of sample b ---------------------------------
+// Channels are those of whole groups: G of them from g0 on, of the sample's allC / allG.
+struct Shape {
+  int B, T, allC, allG, C, G, chunks, rows_per_chunk;
+  // What follows is worked out by the host: a division takes a thread 25 instructions, and what a thread does beside its
+  // rows was as much as 40 rows (16 x 4096 x 320 bf16, 18 rows a thread: 1200 instructions of 2000 in the first pass).
+  int cols, rg, cg, lanes_channels, lanes_chunks;    // columns, rows at a time, channels of a group, threads a group (group_lanes)
+  float inv_cols, inv_cg, inv_T, inv_n;              // inv_n: of a group's T x cg numbers
+  unsigned by_chunks, by_rg;                         // ceil(2^32 / d), see quotient()
+};
+// n / d for n below 2^31 (by = ceil(2^32 / d), 0 for d = 1): the product may be one too large
+__device__ __forceinline__ int quotient(int n, int d, unsigned by) {
+  if (by == 0) return n;
+  const int q = static_cast<int>(__umulhi(static_cast<unsigned>(n), by));
+  return static_cast<unsigned>(q) * static_cast<unsigned>(d) > static_cast<unsigned>(n) ? q - 1 : q;
+}
+// n / d for n below 2^16 by multiplication: (n + 1/2) / d is at least 1 / (2 d) off the next whole number
+__device__ __forceinline__ int small_quotient(int n, float inv) { return static_cast<int>((static_cast<float>(n) + 0.5f) * inv); }
+struct Share { int b, chunk, r0, r1, c0, g0; };
+__device__ __forceinline__ Share share_of(const Shape& h, int b, int slab, int chunk) {
+  Share s;
+  s.b = b;
+  s.chunk = chunk;
+  s.r0 = min(h.T, chunk * h.rows_per_chunk);
+  s.r1 = min(h.T, s.r0 + h.rows_per_chunk);
+  s.c0 = slab * h.C;
+  s.g0 = slab * h.G;
   return s;
+}
+// whole rows, sample by sample
+__device__ __forceinline__ Share share_of(const Shape& h, int block) {
+  const int b = quotient(block, h.chunks, h.by_chunks);
+  return share_of(h, b, 0, block - b * h.chunks);
 }
 // a thread's place: column group `col` of `cols`, row `row` of `rg` rows that the block takes at a time.  Rows of more
 // columns than threads are walked `col`, `col` + GN_THREADS, ...
 struct Place { int cols, rg, col, row; bool on; };
-__device__ __forceinline__ Place place_of(int cols) {
+__device__ __forceinline__ Place place_of(const Shape& h) {
   Place p;
-  p.cols = cols;
-  p.rg = cols < GN_THREADS ? GN_THREADS / cols : 1;
-  p.row = cols < GN_THREADS ? static_cast<int>(threadIdx.x) / cols : 0;
-  p.col = cols < GN_THREADS ? static_cast<int>(threadIdx.x) - p.row * cols : static_cast<int>(threadIdx.x);
+  p.cols = h.cols;
+  p.rg = h.rg;
+  p.row = h.cols < GN_THREADS ? small_quotient(threadIdx.x, h.inv_cols) : 0;
+  p.col = static_cast<int>(threadIdx.x) - p.row * h.cols;
   p.on = p.row < p.rg;
   return p;
 }
 int rows_at_a_time(int cols) { return cols < GN_THREADS ? GN_THREADS / cols : 1; }
 
-// sums over groups of consecutive entries of a shared array: f(group, lane-strided loop body) is run by one warp a group, or by
-// the whole block where there are fewer groups than warps
+// ---- rows on their way ------------------------------------------------------------------------------------
+// A thread reads NT tensors at the same flat indices, a row class's rows one after the other.  With RING its next D rows are
+// copied (cp.async) into slots of shared memory that nobody else touches, so nothing is waited for but the thread's own
+// oldest copy, and what is in flight takes no registers: with loads into registers, two rows ahead, the passes ran at a quarter of
+// the memory's speed (16 x 4096 x 320 bf16: 15, 32, 42 and 46 us from cold).
+template <typename T, int V, int NT, bool RING>
+struct Rows {
+  static constexpr int WIDE = V * static_cast<int>(sizeof(T));                    // bytes a copy
+  static constexpr int SLOT = GN_THREADS * WIDE * NT;
+  static constexpr int D = !RING ? 0 : 32768 / SLOT < 3 ? 3 : 32768 / SLOT > 16 ? 16 : 32768 / SLOT;
+  static constexpr int BYTES = D * SLOT;
+  const T* src[NT];     // where the block's share begins
+  uint32_t slots;       // this thread's first slot
+  uint32_t next;        // the next row to be copied, in elements from there (a share has less than 2^30)
+  uint32_t stride;
+  int left;             // rows not copied yet
+  int slot;
+
+  __device__ __forceinline__ void issue(int d) {
+    if (left > 0) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const uint32_t to = slots + (d * NT + t) * (GN_THREADS * WIDE);
+        if constexpr (WIDE == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src[t] + next) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(src[t] + next) : "memory");
+      }
+      next += stride;
+      --left;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // `rows` rows from `first` on, `step` apart
+  __device__ __forceinline__ void start(uint32_t ring, uint32_t first, uint32_t step, int rows) {
+    next = first;
+    stride = step;
+    left = rows;
+    slot = 0;
+    if constexpr (RING) {
+      slots = ring + threadIdx.x * WIDE;
+#pragma unroll
+      for (int d = 0; d < D; ++d) issue(d);
+    }
+  }
+  // the next row of all tensors
+  __device__ __forceinline__ void take(Nums<V> f[NT]) {
+    if constexpr (RING) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const uint32_t from = slots + (slot * NT + t) * (GN_THREADS * WIDE);
+        Raw<T, V> r;
+        if constexpr (WIDE == 16)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.w.x), "=r"(r.w.y), "=r"(r.w.z), "=r"(r.w.w) : "r"(from) : "memory");
+        else
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r.w) : "r"(from) : "memory");
+        f[t] = unpack_v<T, V>(r);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) f[t] = load_v<T, V>(src[t] + next);
+      next += stride;
+    }
+  }
+  // after the numbers of take() have been used: their slot is filled again
+  __device__ __forceinline__ void advance() {
+    if constexpr (RING) {
+      issue(slot);
+      slot = slot + 1 == D ? 0 : slot + 1;
+    }
+  }
+};
+
+// the rows of a block's share that its thread takes, in the column `col`; none for a thread without a place
+template <typename Stream>
+__device__ __forceinline__ int gn_begin(Stream& in, uint8_t* ring, const Shape& h, const Share& sh, const Place& pl, int V, int col) {
+  const int n = pl.on && col < pl.cols ? quotient(max(0, sh.r1 - sh.r0 - pl.row + pl.rg - 1), pl.rg, h.by_rg) : 0;
+  in.start(smem_u32(ring), static_cast<uint32_t>(pl.row) * h.allC + col * V, static_cast<uint32_t>(pl.rg) * h.allC, n);
+  return n;
+}
+// flat index of a share's first element
+__device__ __forceinline__ size_t share_start(const Shape& h, const Share& sh) { return (static_cast<size_t>(sh.b) * h.T + sh.r0) * h.allC + sh.c0; }
+
+// Sums over each group's entries 0 .. n-1: `lanes` adjacent threads (a power of two) take a group, so that the block works
+// on GN_THREADS / lanes groups at once; every thread of a group gets the sum.  lanes is chosen for the block to be full.
+inline int group_lanes(int G, int n) {
+  int l = 32;
+  while (l > 1 && (l * G > GN_THREADS || l / 2 >= n)) l >>= 1;
+  return l;
+}
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// body(g, k, valid): thread k of the `lanes` of group g (valid: there is such a group); all threads come along for the shuffles
 template <typename Body>
-__device__ __forceinline__ void for_groups(int G, Body body) {
-  const int warp = threadIdx.x >> 5;
-  for (int g = warp; g < G; g += GN_THREADS / 32) body(g);
+__device__ __forceinline__ void for_groups(int G, int lanes, Body body) {
+  const int k = threadIdx.x & (lanes - 1), shift = __popc(lanes - 1), step = GN_THREADS >> shift;
+  for (int g0 = 0; g0 < G; g0 += step) {
+    const int g = g0 + static_cast<int>(threadIdx.x >> shift);
+    body(g < G ? g : G - 1, k, g < G);
+  }
 }
 
 // ---- forward, first pass: mean and sum of squared deviations of every (sample, chunk, group) ------------
-// A thread takes sums about the first number it sees of each channel: the squares then lose nothing to a mean that is
-// large against the spread, and a first number far off the others is itself part of the spread.  What the threads have is
-// put together as (count, mean, squared deviations).
-template <typename T, int V>
-__global__ void __launch_bounds__(GN_THREADS) gn_stats_kernel(const T* __restrict__ x, float2* __restrict__ part, int Tn, int C, int G,
-                                                              int rows_per_chunk, int chunks) {
-  extern __shared__ float2 gn_ent[];       // [rg][C]: mean and squared deviations of a channel over a row class's rows
-  const Span sp = span_of(chunks, rows_per_chunk, Tn);
-  const Place pl = place_of(C / V);
-  pdl_trigger();
-  const T* xb = x + static_cast<size_t>(sp.b) * Tn * C;
-  if (pl.on) {
-    for (int col = pl.col; col < pl.cols; col += GN_THREADS) {
-      float p0[V], s1[V], s2[V];
+// A thread takes its sums about the first number that it sees of a channel: the squares then lose nothing to a mean that is
+// large against the spread, and a first number far off the others is itself part of the spread (n deviations about it lose
+// n 2^-24 of what they add up to, n the few rows of a thread; about one number for the whole chunk the same loss has all its
+// rows for n).  What the threads have is put together as (count, mean, squared deviations).
+template <typename T, int V, bool RING>
+__device__ __forceinline__ void gn_stats(const Shape& h, const Share& sh, const Place& pl, uint8_t* gn_raw, const T* x, float2* part) {
+  using Stream = Rows<T, V, 1, RING>;
+  const int C = h.C, G = h.G;
+  float2* gn_ent = reinterpret_cast<float2*>(gn_raw + Stream::BYTES);       // [rg][C]: mean and squared deviations of a row class, then [0][C] of the chunk
+  const int span_rows = sh.r1 - sh.r0;
+  Stream in;
+  in.src[0] = x + share_start(h, sh);
+  for (int col = pl.col; col < pl.cols && pl.on; col += GN_THREADS) {
+    const int n = gn_begin(in, gn_raw, h, sh, pl, V, col);
+    Nums<V> p0 = n_all<V>(0.f), s1 = p0, s2 = p0, f[1];
+    if (n > 0) {
+      in.take(f);
+      in.advance();
+      p0 = f[0] * -1.f;
+    }
+#pragma unroll 2
+    for (int r = 1; r < n; ++r) {
+      in.take(f);
+      const Nums<V> d = f[0] + p0;
+      in.advance();
+      s1 = s1 + d;
+      s2 = n_fma<V>(d, d, s2);
+    }
+    float fp[V], f1[V], f2[V];
+    n_get<V>(p0, fp);
+    n_get<V>(s1, f1);
+    n_get<V>(s2, f2);
+    const float inv = __fdividef(1.f, static_cast<float>(max(1, n)));
 #pragma unroll
-      for (int e = 0; e < V; ++e) p0[e] = s1[e] = s2[e] = 0.f;
-      const int first = sp.r0 + pl.row;
-      if (first < sp.r1) load_v<T, V>(xb + static_cast<size_t>(first) * C + col * V, p0);
-      int n = first < sp.r1 ? 1 : 0;
-#pragma unroll 4
-      for (int r = first + pl.rg; r < sp.r1; r += pl.rg) {
-        float f[V];
-        load_v<T, V>(xb + static_cast<size_t>(r) * C + col * V, f);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float d = f[e] - p0[e];
-          s1[e] += d;
-          s2[e] = fmaf(d, d, s2[e]);
-        }
-        ++n;
-      }
-      const float inv = n > 0 ? 1.f / n : 0.f;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float m = s1[e] * inv;
-        gn_ent[static_cast<size_t>(pl.row) * C + col * V + e] = make_float2(p0[e] + m, fmaxf(s2[e] - s1[e] * m, 0.f));
-      }
+    for (int e = 0; e < V; ++e) {
+      const float m = f1[e] * inv;
+      gn_ent[static_cast<size_t>(pl.row) * C + col * V + e] = make_float2(m - fp[e], fmaxf(f2[e] - f1[e] * m, 0.f));
     }
   }
   __syncthreads();
-  const int cg = C / G, lane = threadIdx.x & 31, span_rows = sp.r1 - sp.r0;
-  for_groups(G, [&](int g) {
-    const float ref = gn_ent[g * cg].x;
-    float sum = 0.f, cnt = 0.f;
-    for (int k = 0; k < pl.rg; ++k) {
-      const float n = static_cast<float>((span_rows - k + pl.rg - 1) / pl.rg);     // rows of class k (0 from the last row on)
-      if (n <= 0.f) break;
-      for (int c = lane; c < cg; c += 32) { sum = fmaf(n, gn_ent[static_cast<size_t>(k) * C + g * cg + c].x - ref, sum); cnt += n; }
+  // row classes: those before `longer` have one row more than the others
+  const int classes = min(pl.rg, span_rows), base_rows = quotient(span_rows, pl.rg, h.by_rg), longer = span_rows - base_rows * pl.rg;
+  const float inv = 1.f / max(1, span_rows);
+  for (int c = threadIdx.x; c < C; c += GN_THREADS) {
+    const float2 first = gn_ent[c];
+    float sum = 0.f, m2 = first.y;
+    for (int k = 1; k < classes; ++k) sum = fmaf(static_cast<float>(base_rows + (k < longer)), gn_ent[static_cast<size_t>(k) * C + c].x - first.x, sum);
+    const float m = sum * inv;               // the channel's mean, less the first class's
+    m2 = fmaf(static_cast<float>(base_rows + (0 < longer)) * m, m, m2);
+    for (int k = 1; k < classes; ++k) {
+      const float2 v = gn_ent[static_cast<size_t>(k) * C + c];
+      const float d = v.x - first.x - m;
+      m2 += fmaf(static_cast<float>(base_rows + (k < longer)) * d, d, v.y);
     }
-    sum = warp_sum(sum);
-    cnt = warp_sum(cnt);
-    const float mean = ref + sum / cnt;
+    gn_ent[c] = make_float2(first.x + m, m2);
+  }
+  __syncthreads();
+  const int cg = h.cg, lanes = h.lanes_channels;
+  for_groups(G, lanes, [&](int g, int k, bool valid) {
+    const float2* e = gn_ent + g * cg;
+    const float ref = e[0].x;
+    float sum = 0.f;
+    for (int c = k; c < cg; c += lanes) sum += e[c].x - ref;
+    const float mean = fmaf(lanes_sum(sum, lanes), h.inv_cg, ref);
     float m2 = 0.f;
-    for (int k = 0; k < pl.rg; ++k) {
-      const float n = static_cast<float>((span_rows - k + pl.rg - 1) / pl.rg);
-      if (n <= 0.f) break;
-      for (int c = lane; c < cg; c += 32) {
-        const float2 v = gn_ent[static_cast<size_t>(k) * C + g * cg + c];
-        const float d = v.x - mean;
-        m2 += fmaf(n * d, d, v.y);
-      }
+    for (int c = k; c < cg; c += lanes) {
+      const float2 v = e[c];
+      const float d = v.x - mean;
+      m2 += fmaf(span_rows * d, d, v.y);
     }
-    m2 = warp_sum(m2);
-    if (lane == 0) part[(static_cast<size_t>(sp.b) * chunks + sp.chunk) * G + g] = make_float2(mean, m2);
+    m2 = lanes_sum(m2, lanes);
+    if (valid && k == 0) part[(static_cast<size_t>(sh.b) * h.chunks + sh.chunk) * h.allG + sh.g0 + g] = make_float2(mean, m2);
+  });
+}
+
+template <typename T, int V, bool RING>
+__global__ void __launch_bounds__(GN_THREADS, gn_per_sm(false)) gn_stats_kernel(const Shape h, const T* x, float2* part) {
+  extern __shared__ __align__(16) uint8_t gn_raw[];
+  pdl_trigger();
+  gn_stats<T, V, RING>(h, share_of(h, blockIdx.x), place_of(h), gn_raw, x, part);
+}
+
+// floats of a per-channel array in shared memory: what follows it is 16-byte aligned again, whatever C is
+__host__ __device__ __forceinline__ int gn_pad(int C) { return (C + 3) & ~3; }
+
+// ---- per-channel constants in shared memory ----------------------------------------------------------------
+// A thread's column of channels may lie in one group or in several: the constants are laid out by channel, and a thread
+// takes its own into registers.
+template <int V>
+__device__ __forceinline__ Nums<V> take_v(const float* s, int col) {
+  float f[V];
+  if constexpr (V >= 4) {
+#pragma unroll
+    for (int h = 0; h < V / 4; ++h) {
+      const float4 v = *reinterpret_cast<const float4*>(s + col * V + 4 * h);
+      f[4 * h] = v.x; f[4 * h + 1] = v.y; f[4 * h + 2] = v.z; f[4 * h + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = s[col * V + e];
+  }
+  return n_of<V>(f);
+}
+
+// (mean, squared deviations) of a sample's group from its chunks', by `lanes` threads.  (From L2: in a cluster the others' are new.)
+__device__ __forceinline__ float2 gn_moments(const Shape& h, const float2* p, int chunks, int rows_per_chunk, int lanes, int k) {
+  const float ref = __ldcg(p).x;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int i = k; i < chunks; i += lanes) {
+    const int rows = min(rows_per_chunk, h.T - i * rows_per_chunk);
+    if (rows > 0) sum = fmaf(static_cast<float>(rows), __ldcg(p + static_cast<size_t>(i) * h.allG).x - ref, sum);
+  }
+  const float off = lanes_sum(sum, lanes) * h.inv_T;
+  float m2 = 0.f;
+#pragma unroll 4
+  for (int i = k; i < chunks; i += lanes) {
+    const int rows = min(rows_per_chunk, h.T - i * rows_per_chunk);
+    if (rows > 0) {
+      const float2 v = __ldcg(p + static_cast<size_t>(i) * h.allG);
+      const float d = v.x - ref - off;
+      m2 += fmaf(static_cast<float>(rows) * h.cg * d, d, v.y);
+    }
+  }
+  return make_float2(ref + off, lanes_sum(m2, lanes));
+}
+// 1 / sqrt(v), one Newton step behind the approximate instruction
+__device__ __forceinline__ float inv_sqrt(float v) {
+  const float r = rsqrtf(v);
+  return isinf(r) ? r : r * fmaf(-0.5f * v * r, r, 1.5f);
+}
+__device__ __forceinline__ float2 gn_total(const float2* p, int stride, int chunks, int lanes, int k) {
+  float a = 0.f, b = 0.f;
+#pragma unroll 4
+  for (int i = k; i < chunks; i += lanes) { const float2 v = __ldcg(p + static_cast<size_t>(i) * stride); a += v.x; b += v.y; }
+  return make_float2(lanes_sum(a, lanes), lanes_sum(b, lanes));
+}
+// Many chunks a sample (a few large ones): put together once, a block a sample, rather than by every block of the second pass.
+constexpr int GN_MERGE_CHUNKS = 64;
+template <bool MOMENTS>
+__global__ void __launch_bounds__(GN_THREADS) gn_merge_kernel(const Shape h, const float2* part, float2* whole) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x, lanes = h.lanes_chunks;
+  for_groups(h.G, lanes, [&](int g, int k, bool valid) {
+    const float2* p = part + static_cast<size_t>(b) * h.chunks * h.allG + g;
+    const float2 v = MOMENTS ? gn_moments(h, p, h.chunks, h.rows_per_chunk, lanes, k) : gn_total(p, h.allG, h.chunks, lanes, k);
+    if (valid && k == 0) whole[static_cast<size_t>(b) * h.allG + g] = v;
   });
 }
 
 // ---- forward, second pass -------------------------------------------------------------------------------
-template <typename T, int V, bool DROP>
-__global__ void __launch_bounds__(GN_THREADS) gn_apply_kernel(const T* __restrict__ x, const void* __restrict__ gamma, const void* __restrict__ beta,
-                                                              const float2* __restrict__ part, T* __restrict__ y, float* __restrict__ mean,
-                                                              float* __restrict__ rstd, int Tn, int C, int G, int pdt, float eps, int act,
-                                                              int rows_per_chunk, int chunks, int part_rows, int part_chunks, DropKey key) {
-  extern __shared__ float2 gn_stat[];      // [G]: mean, rstd
-  const Span sp = span_of(chunks, rows_per_chunk, Tn);
-  const Place pl = place_of(C / V);
-  const int cg = C / G;
-  pdl_trigger();
-  pdl_wait();
-  for (int g = threadIdx.x; g < G; g += GN_THREADS) {
-    const float2* p = part + static_cast<size_t>(sp.b) * part_chunks * G + g;
-    const float ref = p[0].x;
-    float sum = 0.f;
-    for (int k = 0; k < part_chunks; ++k) sum = fmaf(static_cast<float>(min(part_rows, Tn - k * part_rows)), p[static_cast<size_t>(k) * G].x - ref, sum);
-    const float m = ref + sum / Tn;
-    float m2 = 0.f;
-    for (int k = 0; k < part_chunks; ++k) {
-      const float2 v = p[static_cast<size_t>(k) * G];
-      const float d = v.x - m;
-      m2 += fmaf(static_cast<float>(min(part_rows, Tn - k * part_rows)) * cg * d, d, v.y);
+// shared: mean, rstd by group, then by channel -mean, A = rstd * gamma, beta; z = (x - mean) * A + beta
+struct GnApply { const void *gamma, *beta; float *mean, *rstd; int pdt, act; float eps; };
+// merge_chunks: how many of `part` there are a sample (one, of all rows, behind gn_merge_kernel)
+template <typename T, int V, bool DROP, bool RING, typename Wait>
+__device__ __forceinline__ void gn_apply(const Shape& h, const Share& sh, const Place& pl, uint8_t* gn_raw, const T* x, const float2* part, int merge_chunks,
+                                         T* y, const GnApply& q, const DropKey& key, Wait wait) {
+  using Stream = Rows<T, V, 1, RING>;
+  const int C = h.C, G = h.G, cp = gn_pad(C);
+  float* gn_c = reinterpret_cast<float*>(gn_raw + Stream::BYTES);
+  float *c_mu = gn_c, *c_a = c_mu + cp, *c_b = c_a + cp;
+  float2* stat = reinterpret_cast<float2*>(c_b + cp);
+  Stream in;
+  in.src[0] = x + share_start(h, sh);
+  int n = gn_begin(in, gn_raw, h, sh, pl, V, pl.col);                // (the rows need not wait for their statistics)
+  wait();
+  const int lanes = merge_chunks == h.chunks ? h.lanes_chunks : 1, rows = merge_chunks == h.chunks ? h.rows_per_chunk : h.T;
+  for_groups(G, lanes, [&](int g, int k, bool valid) {
+    const float2 v = gn_moments(h, part + static_cast<size_t>(sh.b) * merge_chunks * h.allG + sh.g0 + g, merge_chunks, rows, lanes, k);
+    if (valid && k == 0) {
+      const float rs = inv_sqrt(fmaf(v.y, h.inv_n, q.eps));
+      stat[g] = make_float2(v.x, rs);
+      if (sh.chunk == 0) {
+        q.mean[static_cast<size_t>(sh.b) * h.allG + sh.g0 + g] = v.x;
+        q.rstd[static_cast<size_t>(sh.b) * h.allG + sh.g0 + g] = rs;
+      }
     }
-    const float rs = 1.0f / sqrtf(m2 / (static_cast<float>(Tn) * cg) + eps);
-    gn_stat[g] = make_float2(m, rs);
-    if (sp.chunk == 0) { mean[sp.b * G + g] = m; rstd[sp.b * G + g] = rs; }
+  });
+  __syncthreads();
+  for (int c = threadIdx.x; c < C; c += GN_THREADS) {
+    const float2 st = stat[small_quotient(c, h.inv_cg)];
+    c_mu[c] = -st.x;
+    c_a[c] = q.gamma != nullptr ? st.y * load_as(q.gamma, q.pdt, sh.c0 + c) : st.y;
+    c_b[c] = q.beta != nullptr ? load_as(q.beta, q.pdt, sh.c0 + c) : 0.f;
   }
   __syncthreads();
   if (!pl.on) return;
   const uint32_t step = DROP ? drop_step(key) : 0;
-  const size_t base = static_cast<size_t>(sp.b) * Tn * C;
+  const size_t start = share_start(h, sh);
+  T* out = y + start;
   for (int col = pl.col; col < pl.cols; col += GN_THREADS) {
-    float mu[V], A[V], Bt[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = col * V + e;
-      const float2 st = gn_stat[c / cg];
-      mu[e] = st.x;
-      A[e] = gamma != nullptr ? st.y * load_as(gamma, pdt, c) : st.y;
-      Bt[e] = beta != nullptr ? load_as(beta, pdt, c) : 0.f;
-    }
+    const Nums<V> mu = take_v<V>(c_mu, col), A = take_v<V>(c_a, col), Bt = take_v<V>(c_b, col);
+    if (col != pl.col) n = gn_begin(in, gn_raw, h, sh, pl, V, col);
+    uint32_t i = static_cast<uint32_t>(pl.row) * h.allC + col * V;
 #pragma unroll 2
-    for (int r = sp.r0 + pl.row; r < sp.r1; r += pl.rg) {
-      const size_t i = base + static_cast<size_t>(r) * C + col * V;
-      float z[V], a[V];
-      load_v<T, V>(x + i, z);
-#pragma unroll
-      for (int e = 0; e < V; ++e) z[e] = fmaf(z[e] - mu[e], A[e], Bt[e]);
-      activate<sizeof(T) == 2, V>(act, z, a);
-      if (DROP) {
-        const uint32_t keep = keep_v<V>(key, step, i);
-#pragma unroll
-        for (int e = 0; e < V; ++e) a[e] = (keep >> e) & 1u ? a[e] * key.scale : 0.f;
-      }
-      store_v<T, V>(y + i, a);
+    for (int r = 0; r < n; ++r, i += in.stride) {
+      Nums<V> f[1];
+      in.take(f);
+      const Nums<V> d = f[0] + mu;
+      in.advance();
+      Nums<V> a = activate<V>(q.act, n_fma<V>(d, A, Bt));
+      if (DROP) a = n_drop<V>(key, step, start + i, a);
+      store_v<T, V>(out + i, a);
     }
   }
+}
+
+template <typename T, int V, bool DROP, bool RING>
+__global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_apply_kernel(const Shape h, const T* x, const float2* part, int merge_chunks, T* y, const GnApply q,
+                                                                 const DropKey key) {
+  extern __shared__ __align__(16) uint8_t gn_raw[];
+  pdl_trigger();
+  // from the back: what the first pass read last is in L2
+  gn_apply<T, V, DROP, RING>(h, share_of(h, gridDim.x - 1 - blockIdx.x), place_of(h), gn_raw, x, part, merge_chunks, y, q, key, [] { pdl_wait(); });
+}
+
+// ---- both passes in one kernel --------------------------------------------------------------------------
+// A cluster of h.chunks blocks takes some groups of one sample, reduces, meets at the cluster's barrier and writes: no
+// block waits for another cluster, and while one cluster's blocks wait others of their SM work.
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ Share cluster_share(const Shape& h) {
+  const int slabs = h.allG / h.G, id = quotient(blockIdx.x, h.chunks, h.by_chunks);
+  return share_of(h, id / slabs, id % slabs, blockIdx.x - id * h.chunks);
+}
+template <typename T, int V, bool DROP, bool RING>
+__global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_fwd_cluster_kernel(const Shape h, const T* x, float2* part, T* y, const GnApply q, const DropKey key) {
+  extern __shared__ __align__(16) uint8_t gn_raw[];
+  const Share sh = cluster_share(h);
+  const Place pl = place_of(h);
+  gn_stats<T, V, RING>(h, sh, pl, gn_raw, x, part);
+  gn_apply<T, V, DROP, RING>(h, sh, pl, gn_raw, x, part, h.chunks, y, q, key, [] { cluster_meet(); });
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------
-// per-channel constants of a thread's column: z = xhat * gamma + beta, xhat = (x - mu) * rs
-template <int V>
-struct Column { float mu[V], rs[V], ga[V], be[V]; };
-template <int V>
-__device__ __forceinline__ void load_column(Column<V>& k, const void* gamma, const void* beta, const float* mean, const float* rstd, int pdt,
-                                            int b, int G, int cg, int col) {
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int c = col * V + e, g = b * G + c / cg;
-    k.mu[e] = __ldg(mean + g);
-    k.rs[e] = __ldg(rstd + g);
-    k.ga[e] = gamma != nullptr ? load_as(gamma, pdt, c) : 1.f;
-    k.be[e] = beta != nullptr ? load_as(beta, pdt, c) : 0.f;
+// shared constants by channel: -mean, A = rstd * gamma, beta
+__device__ __forceinline__ void bwd_constants(float* c_mu, float* c_a, float* c_b, const void* gamma, const void* beta, const float* mean,
+                                              const float* rstd, int pdt, const Shape& h, const Share& sh) {
+  const int C = h.C;
+  for (int c = threadIdx.x; c < C; c += GN_THREADS) {
+    const size_t g = static_cast<size_t>(sh.b) * h.allG + sh.g0 + small_quotient(c, h.inv_cg);
+    c_mu[c] = -__ldg(mean + g);
+    const float rs = __ldg(rstd + g);
+    c_a[c] = gamma != nullptr ? rs * load_as(gamma, pdt, sh.c0 + c) : rs;
+    c_b[c] = beta != nullptr ? load_as(beta, pdt, sh.c0 + c) : 0.f;
   }
 }
-// gz and xhat of V elements at flat index i
-template <typename T, int V, bool DROP>
-__device__ __forceinline__ void gz_xhat(const T* dy, const T* x, size_t i, const Column<V>& k, int act, const DropKey& key, uint32_t step,
-                                        float gz[V], float xh[V]) {
-  float z[V];
-  load_v<T, V>(dy + i, gz);
-  load_v<T, V>(x + i, xh);
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    xh[e] = (xh[e] - k.mu[e]) * k.rs[e];
-    z[e] = fmaf(xh[e], k.ga[e], k.be[e]);
-  }
-  if (DROP) {
-    const uint32_t keep = keep_v<V>(key, step, i);
-#pragma unroll
-    for (int e = 0; e < V; ++e) gz[e] = (keep >> e) & 1u ? gz[e] * key.scale : 0.f;
-  }
-  times_slope<sizeof(T) == 2, V>(act, z, gz);
+// f[0] = dy becomes gz, f[1] = x becomes x - mean, for V elements at flat index i
+template <int V, bool DROP>
+__device__ __forceinline__ void gz_dev(Nums<V> f[2], size_t i, const Nums<V>& mu, const Nums<V>& A, const Nums<V>& Bt, int act, const DropKey& key,
+                                       uint32_t step) {
+  f[1] = f[1] + mu;
+  if (DROP) f[0] = n_drop<V>(key, step, i, f[0]);
+  if (act != FDP_ACT_NONE) f[0] = times_slope<V>(act, n_fma<V>(f[1], A, Bt), f[0]);
 }
 
 // first pass: part[0][b][chunk][c] = sum gz * xhat, part[1] = sum gz; gpart[b][chunk][g] = (sum_c gamma * sum gz, the same with xhat)
-template <typename T, int V, bool DROP>
-__global__ void __launch_bounds__(GN_THREADS) gn_bwd_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, const void* __restrict__ gamma,
-                                                                 const void* __restrict__ beta, const float* __restrict__ mean,
-                                                                 const float* __restrict__ rstd, float* __restrict__ part,
-                                                                 float2* __restrict__ gpart, int B, int Tn, int C, int G, int pdt, int act,
-                                                                 int rows_per_chunk, int chunks, DropKey key) {
-  extern __shared__ float2 gn_sum[];       // [rg][C]: (sum gz, sum gz * xhat) of a row class, then [0][C] of the chunk
-  const Span sp = span_of(chunks, rows_per_chunk, Tn);
-  const Place pl = place_of(C / V);
-  const int cg = C / G;
-  pdl_trigger();
+struct GnBwd { const void *gamma, *beta; const float *mean, *rstd; int pdt, act; };
+template <typename T, int V, bool DROP, bool RING>
+__device__ __forceinline__ void gn_bwd_sums(const Shape& h, const Share& sh, const Place& pl, uint8_t* gn_raw, const T* dy, const T* x, const GnBwd& q,
+                                            float* part, float2* gpart, const DropKey& key) {
+  using Stream = Rows<T, V, 2, RING>;
+  const int C = h.C, G = h.G, cp = gn_pad(C), cg = h.cg;
+  float* gn_c = reinterpret_cast<float*>(gn_raw + Stream::BYTES);
+  float *c_mu = gn_c, *c_a = c_mu + cp, *c_b = c_a + cp;
+  float2* ent = reinterpret_cast<float2*>(gn_c);       // the sums [rg][C] take the constants' place afterwards
+  Stream in;
+  in.src[0] = dy + share_start(h, sh);
+  in.src[1] = x + share_start(h, sh);
+  int n = gn_begin(in, gn_raw, h, sh, pl, V, pl.col);
+  bwd_constants(c_mu, c_a, c_b, q.gamma, q.beta, q.mean, q.rstd, q.pdt, h, sh);
+  __syncthreads();
   const uint32_t step = DROP ? drop_step(key) : 0;
-  const size_t base = static_cast<size_t>(sp.b) * Tn * C;
-  if (pl.on) {
-    for (int col = pl.col; col < pl.cols; col += GN_THREADS) {
-      Column<V> k;
-      load_column<V>(k, gamma, beta, mean, rstd, pdt, sp.b, G, cg, col);
-      float s1[V], s2[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
+  float* wide = gn_c + 3 * cp;                          // rows of more columns than threads: sums apart from the constants
+  const bool apart = pl.cols > GN_THREADS;
+  const size_t start = share_start(h, sh);
+  float s1[V], s2[V];
+  for (int col = pl.col; col < pl.cols && pl.on; col += GN_THREADS) {
+    const Nums<V> mu = take_v<V>(c_mu, col), A = take_v<V>(c_a, col), Bt = take_v<V>(c_b, col);
+    Nums<V> t1 = n_all<V>(0.f), t2 = t1;
+    if (col != pl.col) n = gn_begin(in, gn_raw, h, sh, pl, V, col);
+    uint32_t i = static_cast<uint32_t>(pl.row) * h.allC + col * V;
 #pragma unroll 2
-      for (int r = sp.r0 + pl.row; r < sp.r1; r += pl.rg) {
-        float gz[V], xh[V];
-        gz_xhat<T, V, DROP>(dy, x, base + static_cast<size_t>(r) * C + col * V, k, act, key, step, gz, xh);
+    for (int r = 0; r < n; ++r, i += in.stride) {
+      Nums<V> f[2];
+      in.take(f);
+      gz_dev<V, DROP>(f, start + i, mu, A, Bt, q.act, key, step);
+      in.advance();
+      t1 = t1 + f[0];
+      t2 = n_fma<V>(f[0], f[1], t2);
+    }
+    n_get<V>(t1, s1);
+    n_get<V>(t2, s2);
+    if (apart) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) { s1[e] += gz[e]; s2[e] = fmaf(gz[e], xh[e], s2[e]); }
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) gn_sum[static_cast<size_t>(pl.row) * C + col * V + e] = make_float2(s1[e], s2[e]);
+      for (int e = 0; e < V; ++e) reinterpret_cast<float2*>(wide)[col * V + e] = make_float2(s1[e], s2[e]);
     }
   }
   __syncthreads();
-  const size_t at = (static_cast<size_t>(sp.b) * chunks + sp.chunk) * C, second = static_cast<size_t>(B) * chunks * C;
+  if (apart) {
+    ent = reinterpret_cast<float2*>(wide);
+  } else {
+    if (pl.on) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) ent[static_cast<size_t>(pl.row) * C + pl.col * V + e] = make_float2(s1[e], s2[e]);
+    }
+    __syncthreads();
+  }
+  const size_t at = (static_cast<size_t>(sh.b) * h.chunks + sh.chunk) * h.allC + sh.c0, second = static_cast<size_t>(h.B) * h.chunks * h.allC;
   for (int c = threadIdx.x; c < C; c += GN_THREADS) {
-    float2 t = gn_sum[c];
-    for (int k = 1; k < pl.rg; ++k) { const float2 v = gn_sum[static_cast<size_t>(k) * C + c]; t.x += v.x; t.y += v.y; }
+    float2 t = ent[c];
+    for (int k = 1; k < pl.rg; ++k) { const float2 v = ent[static_cast<size_t>(k) * C + c]; t.x += v.x; t.y += v.y; }
+    t.y *= __ldg(q.rstd + static_cast<size_t>(sh.b) * h.allG + sh.g0 + small_quotient(c, h.inv_cg));
     part[at + c] = t.y;
     part[second + at + c] = t.x;
-    const float ga = gamma != nullptr ? load_as(gamma, pdt, c) : 1.f;
-    gn_sum[c] = make_float2(ga * t.x, ga * t.y);
+    const float ga = q.gamma != nullptr ? load_as(q.gamma, q.pdt, sh.c0 + c) : 1.f;
+    ent[c] = make_float2(ga * t.x, ga * t.y);
   }
   if (gpart == nullptr) return;
   __syncthreads();
-  const int lane = threadIdx.x & 31;
-  for_groups(G, [&](int g) {
-    float a = 0.f, b = 0.f;
-    for (int c = lane; c < cg; c += 32) { const float2 v = gn_sum[g * cg + c]; a += v.x; b += v.y; }
-    a = warp_sum(a);
-    b = warp_sum(b);
-    if (lane == 0) gpart[(static_cast<size_t>(sp.b) * chunks + sp.chunk) * G + g] = make_float2(a, b);
+  const int lanes = h.lanes_channels;
+  for_groups(G, lanes, [&](int g, int k, bool valid) {
+    const float2* e = ent + g * cg;
+    float u = 0.f, v = 0.f;
+    for (int c = k; c < cg; c += lanes) { u += e[c].x; v += e[c].y; }
+    u = lanes_sum(u, lanes);
+    v = lanes_sum(v, lanes);
+    if (valid && k == 0) gpart[(static_cast<size_t>(sh.b) * h.chunks + sh.chunk) * h.allG + sh.g0 + g] = make_float2(u, v);
   });
 }
+template <typename T, int V, bool DROP, bool RING>
+__global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_bwd_sums_kernel(const Shape h, const T* dy, const T* x, const GnBwd q, float* part, float2* gpart,
+                                                                               const DropKey key) {
+  extern __shared__ __align__(16) uint8_t gn_raw[];
+  pdl_trigger();
+  gn_bwd_sums<T, V, DROP, RING>(h, share_of(h, blockIdx.x), place_of(h), gn_raw, dy, x, q, part, gpart, key);
+}
 
-// second pass: dx
-template <typename T, int V, bool DROP>
-__global__ void __launch_bounds__(GN_THREADS) gn_bwd_dx_kernel(const T* __restrict__ dy, const T* __restrict__ x, const void* __restrict__ gamma,
-                                                               const void* __restrict__ beta, const float* __restrict__ mean,
-                                                               const float* __restrict__ rstd, const float2* __restrict__ gpart, T* __restrict__ dx,
-                                                               int Tn, int C, int G, int pdt, int act, int rows_per_chunk, int chunks, DropKey key) {
-  extern __shared__ float2 gn_s[];         // [G]: s1, s2
-  const Span sp = span_of(chunks, rows_per_chunk, Tn);
-  const Place pl = place_of(C / V);
-  const int cg = C / G;
+// per-sample gradients from their chunks: out[tensor][b][c], and the sums of squares of every 32 columns, one block's
+// share: 32 columns of one sample and tensor, one of each warp a column
+__device__ __forceinline__ void gn_psgrad(int piece, float* red, const float* part, float* out, float* sumsq, int chunks, int C) {
+  const int nblk = (C + 31) / 32, sample = piece / nblk, l = threadIdx.x & 31, k0 = threadIdx.x >> 5;
+  const int c = (piece - sample * nblk) * 32 + l;
+  const float* p = part + static_cast<size_t>(sample) * chunks * C + c;
+  float t = 0.f;
+  if (c < C)
+#pragma unroll 8
+    for (int k = k0; k < chunks; k += GN_WARPS) t += p[static_cast<size_t>(k) * C];
+  red[threadIdx.x] = t;
+  __syncthreads();
+  if (k0 == 0) {
+#pragma unroll
+    for (int k = 1; k < GN_WARPS; ++k) t += red[k * 32 + l];
+    if (c < C) out[static_cast<size_t>(sample) * C + c] = t;
+    t = warp_sum(t * t);
+    if (l == 0) sumsq[piece] = t;
+  }
+}
+__global__ void __launch_bounds__(GN_THREADS) gn_psgrad_kernel(const float* part, float* out, float* sumsq, int chunks, int C) {
+  __shared__ float red[GN_THREADS];
   pdl_trigger();
   pdl_wait();
-  const float inv_n = 1.f / (static_cast<float>(Tn) * cg);
-  for (int g = threadIdx.x; g < G; g += GN_THREADS) {
-    const float2* p = gpart + static_cast<size_t>(sp.b) * chunks * G + g;
-    float a = 0.f, b = 0.f;
-    for (int k = 0; k < chunks; ++k) { const float2 v = p[static_cast<size_t>(k) * G]; a += v.x; b += v.y; }
-    gn_s[g] = make_float2(a * inv_n, b * inv_n);
-  }
+  gn_psgrad(blockIdx.x, red, part, out, sumsq, chunks, C);
+}
+// second pass: dx = A * gz - c1 - (x - mean) * c2, c1 = rstd * s1, c2 = rstd^2 * s2
+template <typename T, int V, bool DROP, bool RING, typename Wait>
+__device__ __forceinline__ void gn_bwd_dx(const Shape& h, const Share& sh, const Place& pl, uint8_t* gn_raw, const T* dy, const T* x, const GnBwd& q,
+                                          const float2* gpart, int merge_chunks, T* dx, const DropKey& key, Wait wait) {
+  using Stream = Rows<T, V, 2, RING>;
+  const int C = h.C, G = h.G, cp = gn_pad(C), cg = h.cg;
+  float* gn_c = reinterpret_cast<float*>(gn_raw + Stream::BYTES);
+  float *c_mu = gn_c, *c_a = c_mu + cp, *c_b = c_a + cp, *c_1 = c_b + cp, *c_2 = c_1 + cp;
+  Stream in;
+  in.src[0] = dy + share_start(h, sh);
+  in.src[1] = x + share_start(h, sh);
+  int n = gn_begin(in, gn_raw, h, sh, pl, V, pl.col);
+  wait();
+  bwd_constants(c_mu, c_a, c_b, q.gamma, q.beta, q.mean, q.rstd, q.pdt, h, sh);
+  const float inv_n = h.inv_n;
+  const int lanes = merge_chunks == h.chunks ? h.lanes_chunks : h.lanes_channels;
+  for_groups(G, lanes, [&](int g, int k, bool valid) {
+    const float2 v = gn_total(gpart + static_cast<size_t>(sh.b) * merge_chunks * h.allG + sh.g0 + g, h.allG, merge_chunks, lanes, k);
+    if (valid) {
+      const float rs = __ldg(q.rstd + static_cast<size_t>(sh.b) * h.allG + sh.g0 + g);
+      for (int c = g * cg + k; c < (g + 1) * cg; c += lanes) { c_1[c] = -rs * (v.x * inv_n); c_2[c] = -rs * rs * (v.y * inv_n); }
+    }
+  });
   __syncthreads();
   if (!pl.on) return;
   const uint32_t step = DROP ? drop_step(key) : 0;
-  const size_t base = static_cast<size_t>(sp.b) * Tn * C;
+  const size_t start = share_start(h, sh);
+  T* out = dx + start;
   for (int col = pl.col; col < pl.cols; col += GN_THREADS) {
-    Column<V> k;
-    load_column<V>(k, gamma, beta, mean, rstd, pdt, sp.b, G, cg, col);
-    float s1[V], s2[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) { const float2 s = gn_s[(col * V + e) / cg]; s1[e] = s.x; s2[e] = s.y; }
+    const Nums<V> mu = take_v<V>(c_mu, col), A = take_v<V>(c_a, col), Bt = take_v<V>(c_b, col), k1 = take_v<V>(c_1, col), k2 = take_v<V>(c_2, col);
+    if (col != pl.col) n = gn_begin(in, gn_raw, h, sh, pl, V, col);
+    uint32_t i = static_cast<uint32_t>(pl.row) * h.allC + col * V;
 #pragma unroll 2
-    for (int r = sp.r0 + pl.row; r < sp.r1; r += pl.rg) {
-      const size_t i = base + static_cast<size_t>(r) * C + col * V;
-      float gz[V], xh[V];
-      gz_xhat<T, V, DROP>(dy, x, i, k, act, key, step, gz, xh);
-#pragma unroll
-      for (int e = 0; e < V; ++e) gz[e] = k.rs[e] * (fmaf(k.ga[e], gz[e], -s1[e]) - xh[e] * s2[e]);
-      store_v<T, V>(dx + i, gz);
+    for (int r = 0; r < n; ++r, i += in.stride) {
+      Nums<V> f[2];
+      in.take(f);
+      gz_dev<V, DROP>(f, start + i, mu, A, Bt, q.act, key, step);
+      in.advance();
+      store_v<T, V>(out + i, n_fma<V>(f[0], A, n_fma<V>(f[1], k2, k1)));
     }
   }
 }
 
-template <typename T, int V>
-size_t entry_bytes(int C) { return sizeof(float2) * static_cast<size_t>(rows_at_a_time(C / V)) * C; }
+// The launch has blocks in front that form the per-sample gradients, which need the first pass only: no launch of their own.
+struct GnPsgrad { int pieces; const float* part; float *out, *sumsq; };
+template <typename T, int V, bool DROP, bool RING>
+__global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_bwd_dx_kernel(const Shape h, const T* dy, const T* x, const GnBwd q, const float2* gpart,
+                                                                             int merge_chunks, T* dx, const GnPsgrad ps, const DropKey key) {
+  extern __shared__ __align__(16) uint8_t gn_raw[];
+  pdl_trigger();
+  if (static_cast<int>(blockIdx.x) < ps.pieces) {
+    pdl_wait();
+    gn_psgrad(blockIdx.x, reinterpret_cast<float*>(gn_raw), ps.part, ps.out, ps.sumsq, h.chunks, h.C);
+    return;
+  }
+  gn_bwd_dx<T, V, DROP, RING>(h, share_of(h, gridDim.x - 1 - blockIdx.x), place_of(h), gn_raw, dy, x, q, gpart, merge_chunks, dx, key,
+                              [] { pdl_wait(); });
+}
+// In a cluster every block also forms its part of the sample's gradients: one of h.chunks stretches of the channels.
+template <typename T, int V, bool DROP, bool RING>
+__global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_bwd_cluster_kernel(const Shape h, const T* dy, const T* x, const GnBwd q, float* part,
+                                                                                  float2* gpart, T* dx, const GnPsgrad ps, const DropKey key) {
+  extern __shared__ __align__(16) uint8_t gn_raw[];
+  const Share sh = cluster_share(h);
+  const Place pl = place_of(h);
+  pdl_trigger();
+  gn_bwd_sums<T, V, DROP, RING>(h, sh, pl, gn_raw, dy, x, q, part, gpart, key);
+  __syncthreads();
+  auto gradients = [&] {
+    cluster_meet();
+    if (ps.out == nullptr) return;
+    const int width = (h.C + h.chunks - 1) / h.chunks, first = sh.chunk * width, last = min(h.C, first + width);
+    float sq[2] = {0.f, 0.f};
+    for (int v = threadIdx.x; v < 2 * width; v += GN_THREADS) {
+      const int tensor = v >= width ? 1 : 0, c = first + v - tensor * width;
+      if (c >= last) continue;
+      const size_t row = static_cast<size_t>(tensor) * h.B + sh.b;
+      const float* p = ps.part + row * h.chunks * h.allC + sh.c0 + c;
+      float t = 0.f;
+#pragma unroll 8
+      for (int k = 0; k < h.chunks; ++k) t += __ldcg(p + static_cast<size_t>(k) * h.allC);
+      ps.out[row * h.allC + sh.c0 + c] = t;
+      if (tensor == 0) sq[0] = fmaf(t, t, sq[0]); else sq[1] = fmaf(t, t, sq[1]);
+    }
+    __shared__ float red[32];
+    const int parts = h.allG / h.G * h.chunks, at = sh.g0 / h.G * h.chunks + sh.chunk;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float v = block_sum(sq[t], red);
+      if (threadIdx.x == 0) ps.sumsq[(static_cast<size_t>(t) * h.B + sh.b) * parts + at] = v;
+    }
+  };
+  if (dx != nullptr) gn_bwd_dx<T, V, DROP, RING>(h, sh, pl, gn_raw, dy, x, q, gpart, h.chunks, dx, key, gradients);
+  else gradients();
+}
 
-// (the entries of wide rows take up to 64 KB)
+// clip factors from the sums of squares, clipped sum over the samples, mean, noise: 32 columns of one tensor a block, eight
+// threads a column
+__global__ void __launch_bounds__(GN_THREADS) gn_clip_kernel(const float* psgrad, const float* sumsq, int nparts, float Cc, float clamp, float* norms0,
+                                                             float* norms1, void* out0, void* out1, int B, int C, int out_dt, float inv_div, NoiseKey nk0,
+                                                             NoiseKey nk1) {
+  extern __shared__ __align__(16) uint8_t gn_raw[];
+  float* fac = reinterpret_cast<float*>(gn_raw);      // [B]
+  __shared__ float red[GN_THREADS];
+  const int tensor = blockIdx.y, l = threadIdx.x & 31, k0 = threadIdx.x >> 5, c = blockIdx.x * 32 + l;
+  pdl_wait();
+  for (int b = threadIdx.x; b < B; b += GN_THREADS) {
+    const float* p = sumsq + (static_cast<size_t>(tensor) * B + b) * nparts;
+    float sq = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < nparts; ++i) sq += p[i];
+    const float n = norm_of_sumsq(sq);
+    fac[b] = clip_factor(n, Cc, clamp);
+    float* no = tensor == 0 ? norms0 : norms1;
+    if (blockIdx.x == 0 && no != nullptr) no[b] = n;
+  }
+  __syncthreads();
+  float acc = 0.f;
+  const float* p = psgrad + static_cast<size_t>(tensor) * B * C + c;
+  if (c < C)
+#pragma unroll 8
+    for (int b = k0; b < B; b += GN_WARPS) acc = fmaf(fac[b], p[static_cast<size_t>(b) * C], acc);
+  red[threadIdx.x] = acc;
+  __syncthreads();
+  if (k0 == 0 && c < C) {
+#pragma unroll
+    for (int k = 1; k < GN_WARPS; ++k) acc += red[k * 32 + l];
+    float v = acc * inv_div;
+    const NoiseKey& nk = tensor == 0 ? nk0 : nk1;
+    if (nk.std != 0.f) v += noise_at(nk, c);
+    store_as(tensor == 0 ? out0 : out1, out_dt, c, v);
+  }
+}
+
+// Rows of up to GN_RING_CHANNELS channels leave room for the ring beside their constants (five floats a channel and two
+// a group); longer ones are loaded into registers.
+constexpr int GN_RING_CHANNELS = 4096;
+constexpr size_t GN_SMEM_MOST = GN_MAX_CHANNELS * 24;
+static_assert(GN_SMEM_MOST <= 227 * 1024 && GN_RING_CHANNELS * 20 + 3 * 16384 <= GN_SMEM_MOST, "shared memory of a block");
 template <auto KERNEL>
 bool opt_in(size_t bytes) {
   static bool done[64];
   static std::mutex mu;
-  return bytes <= 48 * 1024 || smem_opt_in(done, mu, KERNEL, GN_MAX_CHANNELS * sizeof(float2));
+  return bytes <= 47 * 1024 || smem_opt_in(done, mu, KERNEL, GN_SMEM_MOST);      // (a kernel may have some of its own)
 }
-
-template <typename T, int V>
-int fwd_typed(const GnArgs& a, const GnPlan& pl, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>(static_cast<size_t>(a.B) * pl.chunks);
-  const size_t ent = entry_bytes<T, V>(a.C), stat = sizeof(float2) * a.G;
-  float2* part = static_cast<float2*>(a.workspace);
-  const DropKey key = a.drop != nullptr ? make_drop_key(a.drop) : DropKey{};
-  if (!opt_in<gn_stats_kernel<T, V>>(ent)) return FDP_ERR_LAUNCH;
-  gn_stats_kernel<T, V><<<grid, GN_THREADS, ent, s>>>(static_cast<const T*>(a.x), part, a.T, a.C, a.G, pl.rows_per_chunk, pl.chunks);
-  note_launch();
-#define FDP_GN_APPLY(DROP)                                                                                                                  \
-  do {                                                                                                                                       \
-    if (!opt_in<gn_apply_kernel<T, V, DROP>>(stat)) return FDP_ERR_LAUNCH;                                                                   \
-    launch_dependent(gn_apply_kernel<T, V, DROP>, dim3(grid), dim3(GN_THREADS), stat, s, static_cast<const T*>(a.x), a.gamma, a.beta, part,  \
-                     static_cast<T*>(a.y), a.mean, a.rstd, a.T, a.C, a.G, a.pdt, a.eps, a.act, pl.rows_per_chunk, pl.chunks,                 \
-                     pl.rows_per_chunk, pl.chunks, key);                                                                                     \
-  } while (0)
-  if (a.drop != nullptr) FDP_GN_APPLY(true); else FDP_GN_APPLY(false);
-#undef FDP_GN_APPLY
+template <auto KERNEL, typename... Args>
+int gn_launch(unsigned grid, size_t smem, bool dependent, cudaStream_t s, Args... args) {
+  if (!opt_in<KERNEL>(smem)) return FDP_ERR_LAUNCH;
+  if (dependent) launch_dependent(KERNEL, dim3(grid), dim3(GN_THREADS), smem, s, args...);
+  else KERNEL<<<grid, GN_THREADS, smem, s>>>(args...);
   note_launch();
   return FDP_OK;
 }
-
-template <typename T, int V, bool DROP>
-int bwd_typed(const GnArgs& a, const GnPlan& pl, float* part, float2* gpart, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>(static_cast<size_t>(a.B) * pl.chunks);
-  const size_t ent = entry_bytes<T, V>(a.C), stat = sizeof(float2) * a.G;
-  const DropKey key = a.drop != nullptr ? make_drop_key(a.drop) : DropKey{};
-  if (!opt_in<gn_bwd_sums_kernel<T, V, DROP>>(ent) || !opt_in<gn_bwd_dx_kernel<T, V, DROP>>(stat)) return FDP_ERR_LAUNCH;
-  gn_bwd_sums_kernel<T, V, DROP><<<grid, GN_THREADS, ent, s>>>(
-      static_cast<const T*>(a.dy), static_cast<const T*>(a.x), a.gamma, a.beta, a.mean, a.rstd, part, a.dx != nullptr ? gpart : nullptr, a.B, a.T,
-      a.C, a.G, a.pdt, a.act, pl.rows_per_chunk, pl.chunks, key);
-  note_launch();
-  if (a.dx != nullptr) {
-    launch_dependent(gn_bwd_dx_kernel<T, V, DROP>, dim3(grid), dim3(GN_THREADS), stat, s, static_cast<const T*>(a.dy), static_cast<const T*>(a.x),
-                     a.gamma, a.beta, a.mean, a.rstd, gpart, static_cast<T*>(a.dx), a.T, a.C, a.G, a.pdt, a.act, pl.rows_per_chunk, pl.chunks, key);
-    note_launch();
+// blocks in clusters of `cluster`
+template <auto KERNEL, typename... Args>
+int gn_launch_clusters(unsigned grid, int cluster, size_t smem, cudaStream_t s, Args... args) {
+  static bool done[64];
+  static std::mutex mu;
+  if (!opt_in<KERNEL>(smem)) return FDP_ERR_LAUNCH;
+  if (cluster > 8) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return FDP_ERR_LAUNCH; }
+    std::lock_guard<std::mutex> lk(mu);
+    if (!done[dev] && cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) { cudaGetLastError(); return FDP_ERR_LAUNCH; }
+    done[dev] = true;
   }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(GN_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, KERNEL, args...) != cudaSuccess) { cudaGetLastError(); return FDP_ERR_LAUNCH; }
+  note_launch();
   return FDP_OK;
 }
 
-template <typename T>
+Shape shape_of(const GnArgs& a, const GnPlan& pl, int V) {
+  Shape h{};
+  h.B = a.B; h.T = a.T; h.allC = a.C; h.allG = a.G;
+  h.C = a.C / pl.slabs; h.G = a.G / pl.slabs;
+  h.chunks = pl.chunks; h.rows_per_chunk = pl.rows_per_chunk;
+  h.cols = h.C / V; h.rg = rows_at_a_time(h.cols); h.cg = a.C / a.G;
+  h.lanes_channels = group_lanes(h.G, h.cg); h.lanes_chunks = group_lanes(h.G, pl.chunks);
+  h.inv_cols = 1.0f / h.cols; h.inv_cg = 1.0f / h.cg; h.inv_T = static_cast<float>(1.0 / a.T);
+  h.inv_n = static_cast<float>(1.0 / (static_cast<double>(a.T) * h.cg));
+  const auto by = [](int d) { return d == 1 ? 0u : static_cast<unsigned>(((1ull << 32) + d - 1) / d); };
+  h.by_chunks = by(pl.chunks); h.by_rg = by(h.rg);
+  return h;
+}
+
+template <typename T, int V, bool DROP, bool RING>
+int fwd_typed(const GnArgs& a, const GnPlan& pl, cudaStream_t s) {
+  constexpr size_t ring = Rows<T, V, 1, RING>::BYTES;
+  const Shape h = shape_of(a, pl, V);
+  const size_t ent = ring + sizeof(float2) * static_cast<size_t>(rows_at_a_time(h.C / V)) * h.C;
+  const size_t con = ring + sizeof(float) * (3 * gn_pad(h.C) + 2 * h.G);
+  float2 *part = reinterpret_cast<float2*>(a.gpart), *whole = reinterpret_cast<float2*>(a.gsum);
+  const DropKey key = a.drop != nullptr ? make_drop_key(a.drop) : DropKey{};
+  const GnApply q{a.gamma, a.beta, a.mean, a.rstd, a.pdt, a.act, a.eps};
+  const unsigned grid = static_cast<unsigned>(static_cast<size_t>(a.B) * pl.slabs * pl.chunks);
+  const T* x = static_cast<const T*>(a.x);
+  T* y = static_cast<T*>(a.y);
+  if (pl.cluster) return gn_launch_clusters<gn_fwd_cluster_kernel<T, V, DROP, RING>>(grid, pl.chunks, ent > con ? ent : con, s, h, x, part, y, q, key);
+  const bool merge = pl.chunks > GN_MERGE_CHUNKS;
+  int st = gn_launch<gn_stats_kernel<T, V, RING>>(grid, ent, false, s, h, x, part);
+  if (st == FDP_OK && merge) st = gn_launch<gn_merge_kernel<true>>(a.B, 0, true, s, h, static_cast<const float2*>(part), whole);
+  if (st == FDP_OK)
+    st = gn_launch<gn_apply_kernel<T, V, DROP, RING>>(grid, con, true, s, h, x, static_cast<const float2*>(merge ? whole : part), merge ? 1 : pl.chunks, y, q, key);
+  return st;
+}
+
+// nparts: sums of squares a sample
+template <typename T, int V, bool DROP, bool RING>
+int bwd_typed(const GnArgs& a, const GnPlan& pl, bool need_dw, int* nparts, cudaStream_t s) {
+  constexpr size_t ring = Rows<T, V, 2, RING>::BYTES;
+  const Shape h = shape_of(a, pl, V);
+  const size_t con = sizeof(float) * 3 * gn_pad(h.C), ent = sizeof(float2) * static_cast<size_t>(rows_at_a_time(h.C / V)) * h.C;
+  const size_t sums = ring + (h.C / V > GN_THREADS ? con + sizeof(float2) * h.C : ent > con ? ent : con);
+  size_t out = ring + sizeof(float) * 5 * gn_pad(h.C);
+  if (out < sizeof(float) * GN_THREADS) out = sizeof(float) * GN_THREADS;
+  float2 *gpart = reinterpret_cast<float2*>(a.gpart), *whole = reinterpret_cast<float2*>(a.gsum);
+  const DropKey key = a.drop != nullptr ? make_drop_key(a.drop) : DropKey{};
+  const GnBwd q{a.gamma, a.beta, a.mean, a.rstd, a.pdt, a.act};
+  const unsigned grid = static_cast<unsigned>(static_cast<size_t>(a.B) * pl.slabs * pl.chunks);
+  const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy);
+  T* dx = static_cast<T*>(a.dx);
+  GnPsgrad ps{0, a.part, need_dw ? a.psgrad : nullptr, a.sumsq};
+  if (pl.cluster) {
+    *nparts = pl.slabs * pl.chunks;
+    return gn_launch_clusters<gn_bwd_cluster_kernel<T, V, DROP, RING>>(grid, pl.chunks, sums > out ? sums : out, s, h, dy, x, q, a.part,
+                                                                       dx != nullptr ? gpart : nullptr, dx, ps, key);
+  }
+  *nparts = ceil_div(a.C, 32);
+  const bool merge = pl.chunks > GN_MERGE_CHUNKS;
+  const int pieces = need_dw ? 2 * a.B * *nparts : 0;
+  int st = gn_launch<gn_bwd_sums_kernel<T, V, DROP, RING>>(grid, sums, false, s, h, dy, x, q, a.part, dx != nullptr ? gpart : nullptr, key);
+  if (st == FDP_OK && dx != nullptr) {
+    if (merge) st = gn_launch<gn_merge_kernel<false>>(a.B, 0, true, s, h, static_cast<const float2*>(gpart), whole);
+    ps.pieces = pieces;
+    if (st == FDP_OK)
+      st = gn_launch<gn_bwd_dx_kernel<T, V, DROP, RING>>(grid + pieces, out, true, s, h, dy, x, q, static_cast<const float2*>(merge ? whole : gpart),
+                                                         merge ? 1 : pl.chunks, dx, ps, key);
+  } else if (st == FDP_OK && need_dw) {
+    st = gn_launch<gn_psgrad_kernel>(pieces, 0, true, s, static_cast<const float*>(a.part), a.psgrad, a.sumsq, pl.chunks, a.C);
+  }
+  return st;
+}
+
+template <typename T, bool DROP>
 int fwd_any(const GnArgs& a, const GnPlan& pl, cudaStream_t s) {
-  return pl.vec && aligned16(a.x) && aligned16(a.y) ? fwd_typed<T, 8>(a, pl, s) : fwd_typed<T, 1>(a, pl, s);
+  constexpr int V = 16 / sizeof(T);
+  const bool aligned = aligned16(a.x) && aligned16(a.y);
+  if (pl.vec == V && aligned) return a.C / pl.slabs <= GN_RING_CHANNELS ? fwd_typed<T, V, DROP, true>(a, pl, s) : fwd_typed<T, V, DROP, false>(a, pl, s);
+  if constexpr (V == 8)
+    if (pl.vec == 2 && aligned && a.C / pl.slabs <= GN_RING_CHANNELS) return fwd_typed<T, 2, DROP, true>(a, pl, s);
+  return fwd_typed<T, 1, DROP, false>(a, pl, s);
+}
+template <typename T, bool DROP>
+int bwd_any(const GnArgs& a, const GnPlan& pl, bool need_dw, int* nparts, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const bool aligned = aligned16(a.x) && aligned16(a.dy) && (a.dx == nullptr || aligned16(a.dx));
+  if (pl.vec == V && aligned) return a.C / pl.slabs <= GN_RING_CHANNELS ? bwd_typed<T, V, DROP, true>(a, pl, need_dw, nparts, s) : bwd_typed<T, V, DROP, false>(a, pl, need_dw, nparts, s);
+  if constexpr (V == 8)
+    if (pl.vec == 2 && aligned && a.C / pl.slabs <= GN_RING_CHANNELS) return bwd_typed<T, 2, DROP, true>(a, pl, need_dw, nparts, s);
+  return bwd_typed<T, 1, DROP, false>(a, pl, need_dw, nparts, s);
 }
 template <typename T>
-int bwd_any(const GnArgs& a, const GnPlan& pl, float* part, float2* gpart, cudaStream_t s) {
-  const bool vec = pl.vec && aligned16(a.x) && aligned16(a.dy) && (a.dx == nullptr || aligned16(a.dx));
-  if (a.drop != nullptr) return vec ? bwd_typed<T, 8, true>(a, pl, part, gpart, s) : bwd_typed<T, 1, true>(a, pl, part, gpart, s);
-  return vec ? bwd_typed<T, 8, false>(a, pl, part, gpart, s) : bwd_typed<T, 1, false>(a, pl, part, gpart, s);
+int fwd_drop(const GnArgs& a, const GnPlan& pl, cudaStream_t s) { return a.drop != nullptr ? fwd_any<T, true>(a, pl, s) : fwd_any<T, false>(a, pl, s); }
+template <typename T>
+int bwd_drop(const GnArgs& a, const GnPlan& pl, bool need_dw, int* nparts, cudaStream_t s) {
+  return a.drop != nullptr ? bwd_any<T, true>(a, pl, need_dw, nparts, s) : bwd_any<T, false>(a, pl, need_dw, nparts, s);
 }
 
 }  // namespace
 
-GnPlan gn_plan(int B, int T, int C) {
-  GnPlan pl;
-  pl.vec = C % 8 == 0;
-  // six blocks an SM, each with at least four rows a thread
-  const int rg = rows_at_a_time(pl.vec ? C / 8 : C);
-  const long long most = (static_cast<long long>(T) + 4 * rg - 1) / (4 * rg);
-  long long chunks = (148 * 6 + B - 1) / B;
-  if (chunks > most) chunks = most;
-  pl.rows_per_chunk = static_cast<int>((T + chunks - 1) / chunks);
+// How the work is cut up.  Must not depend on the device in use, nor on pointers: the workspace query has to agree.
+//
+// Small tensors, where launches are what counts: clusters.  A sample's groups go to `slabs` clusters, its rows to the `chunks`
+// blocks of each, and both passes are one kernel (4 x 64 x 128 fp32, forward and backward 10.6 + 15.7 us, with two kernels 13.4 + 17.8).
+// Others: a kernel a pass over whole rows, which keeps the SMs fuller (16 x 4096 x 320 bf16: 91 us, in clusters of 16 blocks 113
+// to 142), in the number of chunks that takes the fewest (rows a thread + fixed cost of a block) a wave of blocks.
+GnPlan gn_plan(int B, int T, int C, int G, int element, int tensors, bool drop) {
+  constexpr int FIXED_ROWS = 6, SEGMENT = 64;          // rows a thread that a block's fixed cost is worth; bytes of a slab's row
+  constexpr long long PIECE = 96 << 10, SMALL = 2 << 20;
+  const int GN_WAVE = 148 * gn_per_sm(drop);
+  GnPlan pl{};
+  const int wide = 16 / element;
+  pl.vec = C % wide == 0 ? wide : wide == 8 && C % 2 == 0 ? 2 : 1;
+  pl.slabs = 1;
+  const long long sample = static_cast<long long>(T) * C * element * tensors;
+  if (sample * B <= SMALL) {
+    // the fewest slabs (whole groups, whole vectors) whose clusters of up to 16 blocks make a block an SM, or the most there are
+    int best = 1, best_chunks = 1;
+    for (int d = 1; d <= G; ++d) {
+      if (G % d != 0) continue;
+      const int cs = C / d;
+      if (cs % pl.vec != 0 || (d > 1 && cs * element < SEGMENT)) continue;
+      const int most = ceil_div(T, 2 * rows_at_a_time(cs / pl.vec));            // chunks of at least two rows a thread
+      int k = 1;
+      while (k < 16 && 2 * k <= most && (sample / d / k > PIECE || static_cast<long long>(B) * d * k < GN_WAVE)) k *= 2;
+      best = d;
+      best_chunks = k;
+      if (static_cast<long long>(B) * d * k >= GN_WAVE && sample / d / k <= PIECE) break;
+    }
+    pl.cluster = true;
+    pl.slabs = best;
+    pl.chunks = best_chunks;
+    pl.rows_per_chunk = ceil_div(T, best_chunks);
+    return pl;
+  }
+  const int rg = rows_at_a_time(C / pl.vec), most = ceil_div(T, 2 * rg);
+  int best = 1;
+  long long best_cost = -1;
+  for (int waves = 1; waves <= 4; ++waves) {
+    long long ch = static_cast<long long>(waves) * GN_WAVE / B;
+    if (ch < 1) ch = 1;
+    if (ch > most) ch = most;
+    const int rows = ceil_div(T, static_cast<int>(ch)), n = ceil_div(T, rows);
+    const long long w = (static_cast<long long>(B) * n + GN_WAVE - 1) / GN_WAVE;
+    const long long cost = w * (ceil_div(rows, rg) + FIXED_ROWS);
+    if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = n; }
+  }
+  pl.rows_per_chunk = ceil_div(T, best);
   pl.chunks = ceil_div(T, pl.rows_per_chunk);
   return pl;
 }
 
 int gn_fwd(const GnArgs& a, int dt, cudaStream_t s) {
-  const GnPlan pl = gn_plan(a.B, a.T, a.C);
-  if (dt == FDP_F32) return fwd_any<float>(a, pl, s);
-  if (dt == FDP_BF16) return fwd_any<__nv_bfloat16>(a, pl, s);
-  return fwd_any<__half>(a, pl, s);
+  const GnPlan pl = gn_plan(a.B, a.T, a.C, a.G, static_cast<int>(dtype_size(dt)), 1, a.drop != nullptr);
+  if (dt == FDP_F32) return fwd_drop<float>(a, pl, s);
+  if (dt == FDP_BF16) return fwd_drop<__nv_bfloat16>(a, pl, s);
+  return fwd_drop<__half>(a, pl, s);
 }
-int gn_bwd(const GnArgs& a, int dt, float* part, float* gpart, cudaStream_t s) {
-  const GnPlan pl = gn_plan(a.B, a.T, a.C);
-  float2* gp = reinterpret_cast<float2*>(gpart);
-  if (dt == FDP_F32) return bwd_any<float>(a, pl, part, gp, s);
-  if (dt == FDP_BF16) return bwd_any<__nv_bfloat16>(a, pl, part, gp, s);
-  return bwd_any<__half>(a, pl, part, gp, s);
+int gn_sumsq_parts(int C, const GnPlan& pl) { return pl.cluster ? pl.slabs * pl.chunks : ceil_div(C, 32); }
+int gn_bwd(const GnArgs& a, int dt, const fdp_dp_params* p, void* dgamma, void* dbeta, float* norms_gamma, float* norms_beta, cudaStream_t s) {
+  const GnPlan pl = gn_plan(a.B, a.T, a.C, a.G, static_cast<int>(dtype_size(dt)), 2, a.drop != nullptr);
+  const bool need_dw = dgamma != nullptr;
+  int nparts = 0;
+  const int st = dt == FDP_F32 ? bwd_drop<float>(a, pl, need_dw, &nparts, s)
+                 : dt == FDP_BF16 ? bwd_drop<__nv_bfloat16>(a, pl, need_dw, &nparts, s) : bwd_drop<__half>(a, pl, need_dw, &nparts, s);
+  if (st != FDP_OK || !need_dw) return st;
+  const int div = p->batch_divisor > 0 ? p->batch_divisor : a.B;
+  const float inv_div = 1.0f / static_cast<float>(div);
+  const NoiseKey nk0 = make_noise_key(p, p->param_id), nk1 = make_noise_key(p, p->param_id2);
+  if (a.B <= 8192) {
+    launch_dependent(gn_clip_kernel, dim3(ceil_div(a.C, 32), 2), dim3(GN_THREADS), sizeof(float) * a.B, s, a.psgrad, a.sumsq, nparts, p->C,
+                     p->clamp_value, norms_gamma, norms_beta, dgamma, dbeta, a.B, a.C, a.pdt, inv_div, nk0, nk1);
+    note_launch();
+  } else {
+    ln_clip_finalize(a.psgrad, a.sumsq, nparts, p->C, p->clamp_value, a.factors, norms_gamma, norms_beta, dgamma, dbeta, a.B, 1, a.C, a.pdt,
+                     inv_div, nk0, nk1, s);
+  }
+  return FDP_OK;
 }
 
 }  // namespace fdp

@@ -109,8 +109,10 @@ void dropout(const void* x, const void* residual, void* y, size_t n, int dt, con
 
 // ---- group norm, channels last ------------------------------------------------------------------------
 constexpr int GN_MAX_CHANNELS = 8192;
-struct GnPlan { bool vec; int rows_per_chunk, chunks; };
-GnPlan gn_plan(int B, int T, int C);
+struct GnPlan { bool cluster; int vec, slabs, chunks, rows_per_chunk; };
+// `element` bytes, `tensors` that both passes read
+GnPlan gn_plan(int B, int T, int C, int G, int element, int tensors, bool drop);
+int gn_sumsq_parts(int C, const GnPlan& pl);
 struct GnArgs {
   const void *x, *dy, *gamma, *beta;     // gamma, beta may be null (one and zero)
   void *y, *dx;                          // dx may be null
@@ -118,11 +120,11 @@ struct GnArgs {
   int B, T, C, G, act, pdt;
   float eps;
   const fdp_dropout_params* drop;        // null: none
-  void* workspace;                       // forward: float2[B, chunks, G]
+  float *gpart, *gsum;                   // float2[B, chunks, G], float2[B, G]
+  float *part, *psgrad, *sumsq, *factors;      // backward: [2][B][chunks][C], [2][B][C], [2][B][gn_sumsq_parts], [2][B]
 };
 int gn_fwd(const GnArgs& a, int dt, cudaStream_t s);
-// part: [2][B][chunks][C] (of dgamma, then of dbeta), what ln_psgrad_reduce takes; gpart: float2[B, chunks, G]
-int gn_bwd(const GnArgs& a, int dt, float* part, float* gpart, cudaStream_t s);
+int gn_bwd(const GnArgs& a, int dt, const fdp_dp_params* p, void* dgamma, void* dbeta, float* norms_gamma, float* norms_beta, cudaStream_t s);
 
 // ---- e4m3 with a scale for each block of 128 (fdp_fp8.cu) ------------------------------------------------
 inline int fp8_pitch(int n) { return (n + 15) & ~15; }      // bytes of a row

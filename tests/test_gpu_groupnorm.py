@@ -58,9 +58,11 @@ def check(ops, x, dy, gamma, beta, G, act, spec=None, eps=1e-5, pdtype=torch.flo
     xd, dyd = x.to(dev()), dy.to(dev())
     wd, bd = (None, None) if w is None else (w.to(dev()), b.to(dev()))
     gy, st = ops.group_norm_forward(xd, wd, bd, G, eps, activation=act, dropout=spec)
-    # what z is made of: the difference x - mean (rounded against x and the mean), times rstd * gamma, and beta
+    # what z is made of: the difference x - mean (rounded against x and the mean), times rstd * gamma, and beta.  The mean is
+    # a number p of the data plus the mean of x - p, whose roundings are relative to the mean of |x - p| <= std + |p - mean|: over the
+    # threads' several p two standard deviations, which times rstd is 2 -- also where x and the mean are next to zero.
     by = lambda a: a.repeat_interleave(C // G, 1)[:, None]
-    big = (x.double().abs() + by(mean.abs())) * by(rstd) * (1 if w is None else w.double().abs()) + (0 if b is None else b.double().abs())
+    big = ((x.double().abs() + by(mean.abs())) * by(rstd) + 2) * (1 if w is None else w.double().abs()) + (0 if b is None else b.double().abs())
     close(gy, y, big * 1.13 * scale * (1 if keep is None else keep), dtype)
     close(st["mean"], mean, x.double().abs().amax((1, 2))[:, None].expand(B, G), torch.float32)
     close(st["rstd"], rstd, rstd * (1 + (mean * rstd).square()), torch.float32)
@@ -76,7 +78,7 @@ def check(ops, x, dy, gamma, beta, G, act, spec=None, eps=1e-5, pdtype=torch.flo
     n = T * C // G
     grp = lambda a: by(a.reshape(B, T, G, C // G).sum((1, 3)) / n)
     lost = slope_err + border
-    xerr = FP32 * (x.double().abs() + by(mean.abs())) * by(rstd)             # of xhat
+    xerr = FP32 * ((x.double().abs() + by(mean.abs())) * by(rstd) + 2)       # of xhat
     u, gz = want["gz"] * gmul, want["gz"].abs()
     extra = by(rstd) * (lost * gmul + grp(lost * gmul) + xhat.abs() * grp(lost * gmul * xhat.abs() + u.abs() * xerr) + xerr * grp((u * xhat).abs()))
     close(res[0], want["dx"][0], want["dx"][1], dtype, extra)

@@ -1,5 +1,4 @@
 """The operators' formulas and refusals, without a GPU."""
-import pytest
 import torch
 
 from oracle import operators as P
