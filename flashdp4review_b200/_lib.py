@@ -81,9 +81,10 @@ SIGNATURES = {
                            [ctypes.POINTER(DropoutParams), c_void_p, c_size_t, c_void_p]),
     "fdp_fp8_pitch": (c_int, [c_int]),
     "fdp_fp8_quantize": (c_int, [c_void_p] * 3 + [c_int] * 3 + [c_void_p]),
-    "fdp_fp8_quantize_weight": (c_int, [c_void_p] * 4 + [c_int] * 3 + [c_void_p]),
+    "fdp_fp8_exponent_bytes": (c_size_t, [c_int] * 2),
+    "fdp_fp8_quantize_weight": (c_int, [c_void_p] * 6 + [c_int] * 3 + [c_void_p]),
     "fdp_fp8_matmul_workspace_bytes": (c_size_t, [c_int] * 3),
-    "fdp_fp8_matmul": (c_int, [c_void_p] * 3 + [c_int] * 2 + [c_void_p] * 2 + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
+    "fdp_fp8_matmul": (c_int, [c_void_p] * 5 + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
     "fdp_group_norm_bwd_workspace_bytes": (c_size_t, [c_int] * 4),
     "fdp_group_norm_bwd": (c_int, [c_void_p] * 11 + [c_int] * 7 + [ctypes.POINTER(DropoutParams), ctypes.POINTER(DPParams),
                                                                   c_void_p, c_size_t, c_void_p]),

@@ -546,6 +546,8 @@ class Fp8Weight:
     values: object        # float8_e4m3fn [r, c]
     values_t: object      # [c, r]
     scales: object        # float32 [ceil(r / 128), ceil(c / 128)]
+    packed: object        # the scales' exponents as the product of `values` reads them,
+    packed_t: object      # and as that of `values_t` does
     layout: str = "out_in"
 
 
@@ -572,9 +574,9 @@ def fp8_quantize_weight(weight, layout="out_in"):
         raise RuntimeError(f"expected a weight with two dimensions, got {tuple(weight.shape)}")
     if layout not in ("out_in", "in_out"):
         raise ValueError(f"layout must be 'out_in' or 'in_out', got {layout!r}")
-    st, q, qt, scales = host.fp8_quantize_weight(weight.contiguous(), code)
+    st, q, qt, scales, packed, packed_t = host.fp8_quantize_weight(weight.contiguous(), code)
     _lib.check(st, "fdp_fp8_quantize_weight")
-    return Fp8Weight(q, qt, scales, layout)
+    return Fp8Weight(q, qt, scales, packed, packed_t, layout)
 
 
 def _fp8_product(x, weight, bias, transposed, out_dtype):
@@ -583,9 +585,9 @@ def _fp8_product(x, weight, bias, transposed, out_dtype):
     code = _dt(x.dtype)
     if x.numel() == 0:
         raise RuntimeError(f"product with an empty operand {tuple(x.shape)}")
-    w, scales = (weight.values_t, weight.scales.t()) if transposed else (weight.values, weight.scales)
+    w, packed = (weight.values_t, weight.packed_t) if transposed else (weight.values, weight.packed)
     b = None if bias is None else bias.to(x.dtype).contiguous()
-    st, y = host.fp8_matmul(x.contiguous(), w, scales, b, code, _dt(out_dtype or x.dtype))
+    st, y = host.fp8_matmul(x.contiguous(), w, packed, b, code, _dt(out_dtype or x.dtype))
     _lib.check(st, "fdp_fp8_matmul")
     return y
 

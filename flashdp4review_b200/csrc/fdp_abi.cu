@@ -118,14 +118,14 @@ int check_group_norm(int B, int T, int C, int G, int activation, int dtype, int 
   if (C % G != 0 || C > GN_MAX_CHANNELS || static_cast<long long>(B) * T >= (1ll << 31) / 2) return FDP_ERR_SHAPE;
   return check_dropout(drop);
 }
-// workspace of fdp_fp8_matmul: quantised x, its scales, the parts of a K split
-struct Fp8Ws { char* q; float *scales, *parts; size_t bytes; Fp8Plan plan; };
+// workspace of fdp_fp8_matmul: quantised x, its exponents, the parts of a K split
+struct Fp8Ws { char *q, *packed; float* parts; size_t bytes; Fp8Plan plan; };
 Fp8Ws fp8_ws(void* base, int rows, int n, int k) {
   Fp8Ws w;
   w.plan = fp8_plan(rows, n, k);
   Carver c(base);
   w.q = c.take<char>(static_cast<size_t>(rows) * fp8_pitch(k));
-  w.scales = c.take<float>(static_cast<size_t>(ceil_div(k, 128)) * rows);
+  w.packed = c.take<char>(fp8_exponent_bytes(rows, k));
   w.parts = reinterpret_cast<float*>(c.take<char>(w.plan.parts_bytes));
   w.bytes = c.off;
   return w;
@@ -919,6 +919,8 @@ int fdp_group_norm_bwd(const void* dy, const void* x, const void* gamma, const v
 
 int fdp_fp8_pitch(int cols) { return cols <= 0 || cols > (1 << 30) ? 0 : fp8_pitch(cols); }
 
+size_t fdp_fp8_exponent_bytes(int rows, int cols) { return rows <= 0 || cols <= 0 ? 0 : fp8_exponent_bytes(rows, cols); }
+
 int fdp_fp8_quantize(const void* x, void* q, float* scales, int rows, int cols, int dtype, fdp_stream_t stream) {
   NvtxRange nvtx_range("fdp_fp8_quantize");
   if (x == nullptr || q == nullptr || scales == nullptr || rows <= 0 || cols <= 0) return FDP_ERR_ARG;
@@ -927,20 +929,21 @@ int fdp_fp8_quantize(const void* x, void* q, float* scales, int rows, int cols, 
   if (!aligned16(q)) return FDP_ERR_ALIGN;
   const int st = current_device_ok();
   if (st != FDP_OK) return st;
-  fp8_rows(x, q, scales, rows, cols, fp8_pitch(cols), dtype, static_cast<cudaStream_t>(stream));
+  fp8_rows(x, q, nullptr, scales, rows, cols, fp8_pitch(cols), dtype, static_cast<cudaStream_t>(stream));
   FDP_LAUNCH_OK();
   return FDP_OK;
 }
 
-int fdp_fp8_quantize_weight(const void* w, void* q, void* qt, float* scales, int rows, int cols, int dtype, fdp_stream_t stream) {
+int fdp_fp8_quantize_weight(const void* w, void* q, void* qt, float* scales, void* packed, void* packed_t, int rows, int cols, int dtype,
+                            fdp_stream_t stream) {
   NvtxRange nvtx_range("fdp_fp8_quantize_weight");
-  if (w == nullptr || q == nullptr || qt == nullptr || scales == nullptr || rows <= 0 || cols <= 0) return FDP_ERR_ARG;
+  if (w == nullptr || q == nullptr || qt == nullptr || scales == nullptr || packed == nullptr || packed_t == nullptr || rows <= 0 || cols <= 0) return FDP_ERR_ARG;
   if (!valid_dtype(dtype)) return FDP_ERR_DTYPE;
   if (rows > (1 << 30) || cols > (1 << 30) || static_cast<long long>(ceil_div(rows, 128)) * ceil_div(cols, 128) >= (1ll << 31) / 2) return FDP_ERR_SHAPE;
   if (!aligned16(q) || !aligned16(qt)) return FDP_ERR_ALIGN;
   const int st = current_device_ok();
   if (st != FDP_OK) return st;
-  fp8_weight(w, q, qt, scales, rows, cols, fp8_pitch(cols), fp8_pitch(rows), dtype, static_cast<cudaStream_t>(stream));
+  fp8_weight(w, q, qt, scales, packed, packed_t, rows, cols, fp8_pitch(cols), fp8_pitch(rows), dtype, static_cast<cudaStream_t>(stream));
   FDP_LAUNCH_OK();
   return FDP_OK;
 }
@@ -950,24 +953,23 @@ size_t fdp_fp8_matmul_workspace_bytes(int rows, int n, int k) {
   return fp8_ws(nullptr, rows, n, k).bytes;
 }
 
-int fdp_fp8_matmul(const void* x, const void* w, const float* w_scales, int scale_stride_n, int scale_stride_k, const void* bias, void* y,
-                   int rows, int n, int k, int dtype, int out_dtype, void* workspace, size_t workspace_bytes, fdp_stream_t stream) {
+int fdp_fp8_matmul(const void* x, const void* w, const void* w_packed, const void* bias, void* y, int rows, int n, int k, int dtype, int out_dtype,
+                   void* workspace, size_t workspace_bytes, fdp_stream_t stream) {
   NvtxRange nvtx_range("fdp_fp8_matmul");
-  if (x == nullptr || w == nullptr || w_scales == nullptr || y == nullptr || rows <= 0 || n <= 0 || k <= 0) return FDP_ERR_ARG;
+  if (x == nullptr || w == nullptr || w_packed == nullptr || y == nullptr || rows <= 0 || n <= 0 || k <= 0) return FDP_ERR_ARG;
   if (!valid_dtype(dtype) || !valid_dtype(out_dtype)) return FDP_ERR_DTYPE;
   // (tiles are numbered in 31 bits, with up to 148 parts of a K split)
   if (rows > (1 << 30) || n > (1 << 30) || k > (1 << 30) || static_cast<long long>(ceil_div(rows, 128)) * ceil_div(n, 128) >= (1ll << 31) / 256 ||
-      static_cast<long long>(ceil_div(rows, 16)) * ceil_div(k, 512) >= (1ll << 31) / 2)
+      static_cast<long long>(ceil_div(rows, 16)) * ceil_div(k, 512) >= (1ll << 31) / 2 || static_cast<long long>(ceil_div(n, 128)) * ceil_div(k, 512) >= (1ll << 31) / 2)
     return FDP_ERR_SHAPE;
-  if (!aligned16(w)) return FDP_ERR_ALIGN;
+  if (!aligned16(w) || !aligned16(w_packed)) return FDP_ERR_ALIGN;
   int st = current_device_ok();
   if (st != FDP_OK) return st;
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < fdp_fp8_matmul_workspace_bytes(rows, n, k)) return FDP_ERR_WORKSPACE;
   const Fp8Ws ws = fp8_ws(workspace, rows, n, k);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  fp8_rows(x, ws.q, ws.scales, rows, k, fp8_pitch(k), dtype, s);
-  st = fp8_gemm(ws.q, fp8_pitch(k), ws.scales, w, fp8_pitch(k), w_scales, scale_stride_n, scale_stride_k, bias, dtype, y, rows, n, k, out_dtype,
-                ws.parts, ws.plan, s);
+  fp8_rows(x, ws.q, ws.packed, nullptr, rows, k, fp8_pitch(k), dtype, s);
+  st = fp8_gemm(ws.q, fp8_pitch(k), ws.packed, w, fp8_pitch(k), w_packed, bias, dtype, y, rows, n, k, out_dtype, ws.parts, ws.plan, s);
   if (st != FDP_OK) return st;
   FDP_LAUNCH_OK();
   return FDP_OK;

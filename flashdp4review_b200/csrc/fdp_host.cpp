@@ -42,6 +42,7 @@ struct Abi {
   decltype(&fdp_group_norm_bwd_workspace_bytes) group_norm_bwd_workspace_bytes;
   decltype(&fdp_group_norm_bwd) group_norm_bwd;
   decltype(&fdp_fp8_pitch) fp8_pitch;
+  decltype(&fdp_fp8_exponent_bytes) fp8_exponent_bytes;
   decltype(&fdp_fp8_quantize) fp8_quantize;
   decltype(&fdp_fp8_quantize_weight) fp8_quantize_weight;
   decltype(&fdp_fp8_matmul_workspace_bytes) fp8_matmul_workspace_bytes;
@@ -58,7 +59,7 @@ void bind(const std::map<std::string, uint64_t>& fns) {
   FDP_BIND(dropout);
   FDP_BIND(group_norm_fwd_workspace_bytes); FDP_BIND(group_norm_fwd);
   FDP_BIND(group_norm_bwd_workspace_bytes); FDP_BIND(group_norm_bwd);
-  FDP_BIND(fp8_pitch); FDP_BIND(fp8_quantize); FDP_BIND(fp8_quantize_weight); FDP_BIND(fp8_matmul_workspace_bytes); FDP_BIND(fp8_matmul);
+  FDP_BIND(fp8_pitch); FDP_BIND(fp8_exponent_bytes); FDP_BIND(fp8_quantize); FDP_BIND(fp8_quantize_weight); FDP_BIND(fp8_matmul_workspace_bytes); FDP_BIND(fp8_matmul);
 #undef FDP_BIND
 }
 
@@ -416,31 +417,33 @@ py::tuple fp8_quantize_weight(const Tensor& w, int dt) {
   const int64_t rows = w.size(0), cols = w.size(1);
   const Tensor q = fp8_matrix(w, rows, cols), qt = fp8_matrix(w, cols, rows);
   const Tensor scales = new_tensor(w, {(rows + 127) / 128, (cols + 127) / 128}, at::kFloat);
+  const int r = static_cast<int>(rows), c = static_cast<int>(cols);
+  const Tensor packed = new_tensor(w, {static_cast<int64_t>(abi.fp8_exponent_bytes(r, c))}, at::kByte);
+  const Tensor packed_t = new_tensor(w, {static_cast<int64_t>(abi.fp8_exponent_bytes(c, r))}, at::kByte);
   int st;
   {
     py::gil_scoped_release nogil;
-    st = abi.fp8_quantize_weight(ptr(w), ptr(q), ptr(qt), static_cast<float*>(ptr(scales)), static_cast<int>(rows), static_cast<int>(cols), dt, stream(w));
+    st = abi.fp8_quantize_weight(ptr(w), ptr(q), ptr(qt), static_cast<float*>(ptr(scales)), ptr(packed), ptr(packed_t), r, c, dt, stream(w));
   }
-  return py::make_tuple(st, q, qt, scales);
+  return py::make_tuple(st, q, qt, scales, packed, packed_t);
 }
 // x (..., k) times w [n, k]^T in 8 bits
-py::tuple fp8_matmul(const Tensor& x, const Tensor& w, const Tensor& scales, const OptTensor& bias, int dt, int out_dt) {
+py::tuple fp8_matmul(const Tensor& x, const Tensor& w, const Tensor& packed, const OptTensor& bias, int dt, int out_dt) {
   const int64_t k = x.size(-1), n = w.size(0), rows = k > 0 ? x.numel() / k : 0;
-  if (w.device() != x.device() || scales.device() != x.device()) refuse("weight is on another device", w);
+  if (w.device() != x.device() || packed.device() != x.device()) refuse("weight is on another device", w);
   if (w.dim() != 2 || w.size(1) != k || w.scalar_type() != at::kFloat8_e4m3fn || w.stride(1) != 1 || w.stride(0) != abi.fp8_pitch(static_cast<int>(k)))
     refuse("weight does not fit the other operand", w);
-  if (scales.scalar_type() != at::kFloat || scales.dim() != 2 || scales.size(0) != (n + 127) / 128 || scales.size(1) != (k + 127) / 128)
-    refuse("scales do not fit the weight", scales);
+  const int r = static_cast<int>(rows), nn = static_cast<int>(n), kk = static_cast<int>(k);
+  if (packed.scalar_type() != at::kByte || !packed.is_contiguous() || static_cast<size_t>(packed.numel()) != abi.fp8_exponent_bytes(nn, kk))
+    refuse("exponents do not fit the weight", packed);
   if (bias.has_value() && (bias->numel() != n || bias->device() != x.device() || bias->scalar_type() != x.scalar_type())) refuse("bias does not fit the output's columns", *bias);
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor y = with_columns(x, n, out_dt);
-  const int r = static_cast<int>(rows), nn = static_cast<int>(n), kk = static_cast<int>(k);
   const Tensor ws = workspace(x, abi.fp8_matmul_workspace_bytes(r, nn, kk));
   int st;
   {
     py::gil_scoped_release nogil;
-    st = abi.fp8_matmul(ptr(x), ptr(w), static_cast<const float*>(ptr(scales)), static_cast<int>(scales.stride(0)), static_cast<int>(scales.stride(1)),
-                        ptr(bias), ptr(y), r, nn, kk, dt, out_dt, ptr(ws), ws.numel(), stream(x));
+    st = abi.fp8_matmul(ptr(x), ptr(w), ptr(packed), ptr(bias), ptr(y), r, nn, kk, dt, out_dt, ptr(ws), ws.numel(), stream(x));
   }
   return py::make_tuple(st, y);
 }

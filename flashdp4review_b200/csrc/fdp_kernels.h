@@ -128,13 +128,18 @@ int gn_bwd(const GnArgs& a, int dt, const fdp_dp_params* p, void* dgamma, void* 
 
 // ---- e4m3 with a scale for each block of 128 (fdp_fp8.cu) ------------------------------------------------
 inline int fp8_pitch(int n) { return (n + 15) & ~15; }      // bytes of a row
-void fp8_rows(const void* x, void* q, float* scales, int rows, int cols, int pitch, int dt, cudaStream_t s);
-void fp8_weight(const void* w, void* q, void* qt, float* scales, int rows, int cols, int pitch, int pitch_t, int dt, cudaStream_t s);
+inline size_t fp8_exponent_bytes(int rows, int cols) {      // units of 128 rows x 512 columns
+  return static_cast<size_t>(ceil_div(rows, 128)) * ceil_div(cols, 512) * 512;
+}
+// packed, scales: may be null
+void fp8_rows(const void* x, void* q, void* packed, float* scales, int rows, int cols, int pitch, int dt, cudaStream_t s);
+void fp8_weight(const void* w, void* q, void* qt, float* scales, void* packed, void* packed_t, int rows, int cols, int pitch, int pitch_t, int dt,
+                cudaStream_t s);
 struct Fp8Plan { int ctas, bn, split; size_t parts_bytes; };
 Fp8Plan fp8_plan(int M, int N, int K);
 // out[M, N] = a[M, K] w[N, K]^T (+ bias), both in e4m3; follows the kernel that quantised `a` in the stream
-int fp8_gemm(const void* a, int pitch_a, const float* sa, const void* w, int pitch_w, const float* sw, int sw_n, int sw_k, const void* bias,
-             int bias_dt, void* out, int M, int N, int K, int out_dt, float* parts, const Fp8Plan& pl, cudaStream_t s);
+int fp8_gemm(const void* a, int pitch_a, const void* sa, const void* w, int pitch_w, const void* sw, const void* bias, int bias_dt, void* out, int M,
+             int N, int K, int out_dt, float* parts, const Fp8Plan& pl, cudaStream_t s);
 
 // ---- LayerNorm -----------------------------------------------------------------------------------
 struct LnPlan { int tpr, cpt, cw, rows_per_block, chunks; bool vec; };

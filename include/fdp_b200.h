@@ -356,19 +356,22 @@ int fdp_group_norm_bwd(const void* dy, const void* x, const void* gamma, const v
  * fdp_fp8_quantize: activations and gradients, blocks of 1 x 128, so that no scale mixes rows (samples).
  *   x [rows,cols] in `dtype` -> q [rows, pitch(cols)] bytes, scales float[ceil(cols / 128)][rows].
  * fdp_fp8_quantize_weight: blocks of 128 x 128, as it lies and transposed (each product contracts over adjacent bytes).
- *   w [rows,cols] -> q [rows, pitch(cols)], qt [cols, pitch(rows)], scales float[ceil(rows / 128)][ceil(cols / 128)].
+ *   w [rows,cols] -> q [rows, pitch(cols)], qt [cols, pitch(rows)], scales float[ceil(rows / 128)][ceil(cols / 128)], and
+ *   packed / packed_t, fdp_fp8_exponent_bytes(rows, cols) and (cols, rows) bytes: the scales' exponents (+ 127) as
+ *   fdp_fp8_matmul reads them, in units of 128 rows x 512 columns, 512 bytes, a row r's four at (r % 32) * 16 + r / 32 * 4,
+ *   units of 128 rows one behind the other.  Bytes that stand for no number are not written.
  * fdp_fp8_matmul: y[rows,n] = quantised(x[rows,k]) * w[n,k]^T (+ bias[n]), accumulated in fp32, rounded once; x and bias in
- *   `dtype`, y in `out_dtype`, w [n, pitch(k)] bytes whose scale of block (i, j) (128 rows i, 128 columns j) is
- *   w_scales[i * scale_stride_n + j * scale_stride_k].  The forward product of a layer is this with its weight [out,in],
- *   its input gradient with the weight transposed.  w 16-byte aligned.
+ *   `dtype`, y in `out_dtype`, w [n, pitch(k)] bytes, w_packed its exponents.  The forward product of a layer is this with
+ *   its weight [out,in], its input gradient with the weight transposed.  w and w_packed 16-byte aligned.
  */
 int fdp_fp8_pitch(int cols);
+size_t fdp_fp8_exponent_bytes(int rows, int cols);
 int fdp_fp8_quantize(const void* x, void* q, float* scales, int rows, int cols, int dtype, fdp_stream_t stream);
-int fdp_fp8_quantize_weight(const void* w, void* q, void* qt, float* scales, int rows, int cols, int dtype, fdp_stream_t stream);
+int fdp_fp8_quantize_weight(const void* w, void* q, void* qt, float* scales, void* packed, void* packed_t, int rows,
+                            int cols, int dtype, fdp_stream_t stream);
 size_t fdp_fp8_matmul_workspace_bytes(int rows, int n, int k);
-int fdp_fp8_matmul(const void* x, const void* w, const float* w_scales, int scale_stride_n, int scale_stride_k,
-                   const void* bias, void* y, int rows, int n, int k, int dtype, int out_dtype, void* workspace,
-                   size_t workspace_bytes, fdp_stream_t stream);
+int fdp_fp8_matmul(const void* x, const void* w, const void* w_packed, const void* bias, void* y, int rows, int n, int k,
+                   int dtype, int out_dtype, void* workspace, size_t workspace_bytes, fdp_stream_t stream);
 
 #ifdef __cplusplus
 }
