@@ -515,6 +515,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         }
       }
       if (!ok) break;
+      const int row0 = m0 + quarter * 32;
+      if (row0 >= args.M) continue;
       if (args.split > 1) {
         float* dst = args.parts + ((static_cast<size_t>(u) * CTAS + cta_rank) * 8 + ew) * (WC * 32);
 #pragma unroll
@@ -525,8 +527,6 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 make_float4(acc_r[c4 * 32 + 4 * j], acc_r[c4 * 32 + 4 * j + 1], acc_r[c4 * 32 + 4 * j + 2], acc_r[c4 * 32 + 4 * j + 3]);
         continue;
       }
-      const int row0 = m0 + quarter * 32;
-      if (row0 >= args.M) continue;
 #pragma unroll
       for (int c4 = 0; c4 < WC / 32; ++c4) {
         const int n = nw + c4 * 32;
@@ -712,20 +712,22 @@ void fp8_weight(const void* w, void* q, void* qt, float* scales, void* packed, v
   else weight_typed<__half>(w, b, bt, scales, p, pt, rows, cols, pitch, pitch_t, s);
 }
 
+// Pair tiles of 256 x 256, single CTAs' of 128 x 128, or those cut along K, whichever is expected to take least: a K block of
+// either tile takes about 0.27 us (the pair's is the tensor cores' time, the small tile's the time of its 32 KB from L2), a
+// tile 1.6 us beside them, the parts of a cut their way to L2 and back and a launch to add them up.
 Fp8Plan fp8_plan(int M, int N, int K) {
-  Fp8Plan pl;
+  constexpr double BLOCK = 0.27, TILE = 1.6, JOIN = 3.0, PARTS_BYTES_A_US = 5e6;
   const int kb = ceil_div(K, 128);
-  const long long pairs = static_cast<long long>(ceil_div(M, 256)) * ceil_div(N, 256);
-  // pair tiles where they fill the GPU, else single CTAs' tiles, cut along K where even those are few
-  if (pairs >= 74) { pl.ctas = 2; pl.bn = 256; pl.split = 1; }
-  else {
-    pl.ctas = 1; pl.bn = 128;
-    const long long tiles = static_cast<long long>(ceil_div(M, 128)) * ceil_div(N, 128);
-    long long split = 148 / tiles;
-    if (split > kb / 4) split = kb / 4;
-    pl.split = split < 1 ? 1 : static_cast<int>(split);
+  const long long pairs = static_cast<long long>(ceil_div(M, 256)) * ceil_div(N, 256), tiles = static_cast<long long>(ceil_div(M, 128)) * ceil_div(N, 128);
+  Fp8Plan pl{2, 256, 1, 0};
+  double best = static_cast<double>((pairs + 73) / 74) * (kb * BLOCK + TILE);
+  for (int split = 1; split <= 16 && split <= kb; split *= 2) {
+    const double rows = M < 128 ? (M + 31) / 32 * 32 : 128;
+    const double parts = split > 1 ? static_cast<double>(tiles) * split * rows * 128 * 4 : 0.0;
+    const double cost = static_cast<double>((tiles * split + 147) / 148) * (ceil_div(kb, split) * BLOCK + TILE) + (split > 1 ? JOIN + 2 * parts / PARTS_BYTES_A_US : 0.0);
+    if (cost < best) { best = cost; pl = Fp8Plan{1, 128, split, 0}; }
   }
-  pl.parts_bytes = pl.split > 1 ? static_cast<size_t>(ceil_div(M, F8_BM * pl.ctas)) * ceil_div(N, pl.bn) * pl.split * pl.ctas * F8_BM * pl.bn * sizeof(float) : 0;
+  if (pl.split > 1) pl.parts_bytes = static_cast<size_t>(tiles) * pl.split * F8_BM * pl.bn * sizeof(float);
   return pl;
 }
 

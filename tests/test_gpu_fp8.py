@@ -1,9 +1,11 @@
 """Products in e4m3 with a scale for each block of 128: quantisation bit for bit, products against float64.
 
-Tolerance of a product: products of two e4m3 numbers are exact in fp32.  One matrix instruction adds 32 of them and the
-accumulator, each cut off at no less than 24 bits below the largest: 33 * 2^-24 of the sum of their magnitudes; a block of 128 takes
-four; then one fp32 rounding a block, the bias's and the last.  (48 + blocks) * 2^-24 of the sum of all magnitudes, and half a
-step of the output type.
+Tolerance of a product: products of two e4m3 numbers are exact in fp32, and so are powers of two as scales.  One matrix
+instruction adds 32 products to the accumulator, each cut off at no less than 24 bits below the largest of them, which is at most
+the sum of all magnitudes: products lose 33 * 2^-24 of what their own instruction adds, 33 * 2^-24 of the sum over all; the accumulator
+one bit of its last place, 2^-23 of the sum, in each of four instructions for every 128 numbers, of which at most 8 * 128 go by for an
+fp32 output before an accumulator starts anew (and is added with one rounding); then the bias's and the last rounding.
+(48 + 8 * blocks) * 2^-24 of the sum of all magnitudes, at most 8 blocks and one more a chain for fp32, and half a step of the output type.
 """
 import math
 
@@ -78,7 +80,9 @@ def check(ops, M, N, K, dtype, out_dtype=None, bias=True, layout="out_in", seed=
         assert got.dtype == t
         want = a @ m + extra
         mag = a.abs() @ m.abs() + (extra.abs() if b is not None and got is y else 0.0)
-        tol = torch.finfo(t).eps / 2 * want.abs() + (48 + -(-k // 128)) * 2.0 ** -24 * mag + torch.finfo(t).smallest_normal * torch.finfo(t).eps
+        blocks = -(-k // 128)
+        lost = 48 + (8 * blocks if t != torch.float32 else 8 * min(blocks, 8) + blocks / 8)
+        tol = torch.finfo(t).eps / 2 * want.abs() + lost * 2.0 ** -24 * mag + torch.finfo(t).smallest_normal * torch.finfo(t).eps
         err = (got.double() - want).abs()
         assert (err <= tol).all(), (err / tol).max()
 
