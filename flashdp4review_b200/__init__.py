@@ -11,9 +11,9 @@ from .layers.dropout import DPDropout
 from .api.wrap_model import wrap_with_flashdp_layers, dp_supported_modules
 from .runtime import (manual_seed, set_data_parallel, set_input_grad_impl, set_accumulation, accumulate,
                       noise_state, set_noise_state, check_device_status, clear_device_status, sm_reservation,
-                      set_fp32_mode, fp32_mode, use_device_noise_step, advance_noise_step)
+                      set_fp32_mode, fp32_mode, use_device_noise_step, advance_noise_step, set_fp8_products, fp8_products)
 
 __all__ = ["DPLinear", "DPLayerNorm", "DPConv1D", "DPGroupNorm", "DPDropout", "wrap_with_flashdp_layers", "dp_supported_modules",
            "manual_seed", "set_data_parallel", "set_input_grad_impl", "set_accumulation", "accumulate",
            "noise_state", "set_noise_state", "check_device_status", "clear_device_status", "sm_reservation", "set_fp32_mode", "fp32_mode",
-           "use_device_noise_step", "advance_noise_step"]
+           "use_device_noise_step", "advance_noise_step", "set_fp8_products", "fp8_products"]

@@ -230,6 +230,12 @@ def library_product_ok(dtype, rows, K, N):
     return native_product_ok(dtype, rows, K, N) or wide_product_ok(dtype, rows, K, N)
 
 
+def fp8_product_ok(dtype, rows, K, N):
+    """Whether a DP layer runs its forward / input-gradient product [rows, K] x [K, N] in 8 bits."""
+    return (runtime.fp8_products() and runtime.input_grad_impl() != "library" and dtype in _DT and rows >= 128 and K >= 64
+            and N >= 64)
+
+
 def fp32_product_flags():
     """flags of a layer's forward product, of which fp32 takes all"""
     flags = _lib.FDP_GEMM_SPLIT_K | _lib.FDP_PAD_16BIT

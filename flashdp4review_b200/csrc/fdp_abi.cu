@@ -863,7 +863,7 @@ int fdp_dropout(const void* x, const void* residual, void* y, size_t n, int dtyp
 }
 
 size_t fdp_group_norm_fwd_workspace_bytes(int B, int T, int C, int G) {
-  if (B <= 0 || T <= 0 || C <= 0 || G <= 0) return 0;
+  if (B <= 0 || T <= 0 || C <= 0 || G <= 0 || C % G != 0 || C > GN_MAX_CHANNELS) return 0;
   return gn_ws(nullptr, B, T, C, G, false).bytes;
 }
 
@@ -887,7 +887,7 @@ int fdp_group_norm_fwd(const void* x, const void* gamma, const void* beta, void*
 }
 
 size_t fdp_group_norm_bwd_workspace_bytes(int B, int T, int C, int G) {
-  if (B <= 0 || T <= 0 || C <= 0 || G <= 0) return 0;
+  if (B <= 0 || T <= 0 || C <= 0 || G <= 0 || C % G != 0 || C > GN_MAX_CHANNELS) return 0;
   return gn_ws(nullptr, B, T, C, G, true).bytes;
 }
 

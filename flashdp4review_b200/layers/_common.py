@@ -104,9 +104,9 @@ _native = None
 
 def native_nodes(input):
     """The call layer with the layers' autograd nodes, or None where the Function classes take the call: tensors that
-    are not on a GPU, and torch.jit.trace, which records a Function but would take a node's output for a constant."""
+    are not on a GPU, products in 8 bits, and torch.jit.trace, which records a Function but would take a node's output for a constant."""
     global _native
-    if not input.is_cuda or torch._C._get_tracing_state() is not None:
+    if not input.is_cuda or runtime.fp8_products() or torch._C._get_tracing_state() is not None:
         return None
     if _native is None:
         host = _lib.host()

@@ -44,6 +44,10 @@ class _DPConv1DFunc(Function):
         ctx.save_for_backward(bias, x, weight, w if dt is not None else None)
         ctx.layer = layer
         ctx.input_dtype = input.dtype
+        ctx.fp8 = None
+        if x.is_cuda and ops.fp8_product_ok(x.dtype, x.numel() // x.shape[-1], w.shape[0], w.shape[1]):
+            ctx.fp8 = ops.fp8_quantize_weight(weight, "in_out")     # for the input gradient too
+            return ops.fp8_linear_forward(x, ctx.fp8, bias)
         if x.is_cuda and ops.library_product_ok(
                 x.dtype, x.numel() // x.shape[-1], w.shape[0], w.shape[1]):
             return ops.linear_forward(x, w, bias, "in_out")     # library GEMM, bias added in its epilogue
@@ -69,9 +73,12 @@ class _DPConv1DFunc(Function):
                 grad_bias = None
             need_db = False
 
-        native_dx = need_dx and ops.library_product_ok(
+        eight_bits = need_dx and ctx.fp8 is not None
+        native_dx = need_dx and not eight_bits and ops.library_product_ok(
             g3.dtype, g3.numel() // g3.shape[-1], w_for_dx.shape[1], w_for_dx.shape[0])
-        if need_dx and not native_dx:
+        if eight_bits:
+            grad_input = ops.fp8_linear_input_grad(g3, ctx.fp8, out_dtype=ctx.input_dtype)
+        elif need_dx and not native_dx:
             grad_input = g3 @ w_for_dx.to(g3.dtype).t()
 
         if native_dx or need_dw or need_db:

@@ -25,6 +25,7 @@ class _Run:
     # kernels (GPT-2-medium on two GPUs: 95.1 ms per step without a reservation, 97.1 ms with 12 SMs)
     reserve_sms = int(os.environ.get("FDP_DP_RESERVE_SMS", "0"))
     fp32_mode = "tensor"          # "tensor": three bf16 tensor-core products where the shape allows; "exact": fp32 FMA kernels
+    fp8_products = False          # forward / input-gradient products in e4m3: see set_fp8_products
     input_grad_impl = "auto"      # forward / input-gradient products of the DP layers: see set_input_grad_impl
     micro_index = 0               # gradient accumulation: which micro-step of `micro_steps` runs now
     micro_steps = 1
@@ -224,6 +225,20 @@ def set_input_grad_impl(name: str):
 
 def input_grad_impl():
     return _run.input_grad_impl
+
+
+def set_fp8_products(on: bool = True):
+    """Forward and input-gradient products of DPLinear and DPConv1D in 8-bit floating point (e4m3, one power-of-two scale for
+    each block of 128): about twice the 16-bit rate, each number rounded to four significant bits.  Inputs and upstream gradients
+    have a scale for each row and 128 columns, so nothing of one sample reaches another and the clipping bounds what it did; the
+    weight, quantised in every forward, one for each 128 x 128 block.  The weight and bias gradients, with their norms, factors
+    and noise, stay what they are without.  Products of fewer than 128 rows or 64 columns on either side do too, and all of
+    them under set_input_grad_impl("library")."""
+    _run.fp8_products = bool(on)
+
+
+def fp8_products():
+    return _run.fp8_products
 
 
 def next_param_id() -> int:
