@@ -144,38 +144,28 @@ __device__ __forceinline__ float rcp(float v) {
   return r;
 }
 constexpr float LOG2E = 1.4426950408889634f, SQRT_2_PI = 0.7978845608028654f, INV_SQRT_2PI = 0.3989422804014327f, SQRT_HALF = 0.7071067811865476f;
-// 1 / (1 + 2^u).  Two reciprocals come from one, 1 / a = b / (a b): the special-function units, a quarter of an issue slot
-// wide, would otherwise be what bounds the passes (21 M elements x 2 of them: 9.4 us, 7 so).  u is held to 60, where the result is
-// 2^-60, so that a product of two is finite, also where one is a NaN (whose activation is one all the same, being a multiple of z).
+// 1 / (1 + 2^u); 2^u may be infinite.  (Tried: two reciprocals out of one, 1 / a = b / (a b), to spare the special-function
+// units.  They are not what bounds the passes, 16 instructions of eight cycles for every eight numbers; holding u down so
+// that a product of two stays finite cost more issue slots than it saved.)
 template <int V> __device__ __forceinline__ Nums<V> n_sigmoid2(const Nums<V>& u) {
   float a[V];
   n_get<V>(u, a);
 #pragma unroll
-  for (int e = 0; e < V; ++e) a[e] = ex2(fminf(a[e], 60.f));
-  if constexpr (V == 1) {
-    return Nums<1>{rcp(1.f + a[0])};
-  } else {
-    Nums<V> s;
-    const pair_t one = pair_of(1.f, 1.f);
+  for (int e = 0; e < V; ++e) a[e] = ex2(a[e]);
+  n_get<V>(n_of<V>(a) + n_all<V>(1.f), a);
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      float x, y;
-      pair_get(pair_add(pair_of(a[2 * i], a[2 * i + 1]), one), x, y);
-      const float r = rcp(x * y);
-      s.p[i] = pair_of(y * r, x * r);
-    }
-    return s;
-  }
+  for (int e = 0; e < V; ++e) a[e] = rcp(a[e]);
+  return n_of<V>(a);
 }
 // gelu_tanh: (1 + tanh w) / 2 = 1 / (1 + e^(-2 w)), which loses nothing where tanh w is near -1; w = sqrt(2/pi) (z + 0.044715 z^3)
 template <int V> __device__ __forceinline__ Nums<V> n_gelu_half(const Nums<V>& z) {
   constexpr float K = -2.f * SQRT_2_PI * LOG2E;
   return n_sigmoid2<V>(n_fma<V>(z * z, n_all<V>(K * 0.044715f), n_all<V>(K)) * z);
 }
-// act(z)
-template <int V>
-__device__ __forceinline__ Nums<V> activate(int act, const Nums<V>& z) {
-  switch (act) {
+// act(z).  The activation is a constant of the loop over rows: a choice inside it would keep the instructions of two rows apart.
+template <int ACT, int V>
+__device__ __forceinline__ Nums<V> activate(const Nums<V>& z) {
+  switch (ACT) {
     case FDP_ACT_RELU: {
       float f[V];
       n_get<V>(z, f);
@@ -198,10 +188,22 @@ __device__ __forceinline__ Nums<V> activate(int act, const Nums<V>& z) {
       return z;
   }
 }
-// g * act'(z)
-template <int V>
-__device__ __forceinline__ Nums<V> times_slope(int act, const Nums<V>& z, const Nums<V>& g) {
+// body(Constant) of an activation known at run time
+template <int N> struct Constant { static constexpr int value = N; };
+template <typename Body>
+__device__ __forceinline__ void with_activation(int act, Body body) {
   switch (act) {
+    case FDP_ACT_RELU: body(Constant<FDP_ACT_RELU>{}); break;
+    case FDP_ACT_SILU: body(Constant<FDP_ACT_SILU>{}); break;
+    case FDP_ACT_GELU: body(Constant<FDP_ACT_GELU>{}); break;
+    case FDP_ACT_GELU_TANH: body(Constant<FDP_ACT_GELU_TANH>{}); break;
+    default: body(Constant<FDP_ACT_NONE>{});
+  }
+}
+// g * act'(z)
+template <int ACT, int V>
+__device__ __forceinline__ Nums<V> times_slope(const Nums<V>& z, const Nums<V>& g) {
+  switch (ACT) {
     case FDP_ACT_RELU: {
       float f[V], h[V];
       n_get<V>(z, f);
@@ -281,12 +283,13 @@ __device__ __forceinline__ Place place_of(const Shape& h) {
 int rows_at_a_time(int cols) { return cols < GN_THREADS ? GN_THREADS / cols : 1; }
 
 // ---- rows on their way ------------------------------------------------------------------------------------
-// A thread reads NT tensors at the same flat indices, a row class's rows one after the other.  With RING its next D rows are
-// copied (cp.async) into slots of shared memory that nobody else touches, so nothing is waited for but the thread's own
+// A thread reads NT tensors at the same flat indices, a row class's rows one after the other.  Where they are vectors its next D
+// rows are copied (cp.async) into slots of shared memory that nobody else touches, so nothing is waited for but the thread's own
 // oldest copy, and what is in flight takes no registers: with loads into registers, two rows ahead, the passes ran at a quarter of
 // the memory's speed (16 x 4096 x 320 bf16: 15, 32, 42 and 46 us from cold).
-template <typename T, int V, int NT, bool RING>
+template <typename T, int V, int NT>
 struct Rows {
+  static constexpr bool RING = V > 1;
   static constexpr int WIDE = V * static_cast<int>(sizeof(T));                    // bytes a copy
   static constexpr int SLOT = GN_THREADS * WIDE * NT;
   static constexpr int D = !RING ? 0 : 32768 / SLOT < 3 ? 3 : 32768 / SLOT > 16 ? 16 : 32768 / SLOT;
@@ -388,9 +391,9 @@ __device__ __forceinline__ void for_groups(int G, int lanes, Body body) {
 // large against the spread, and a first number far off the others is itself part of the spread (n deviations about it lose
 // n 2^-24 of what they add up to, n the few rows of a thread; about one number for the whole chunk the same loss has all its
 // rows for n).  What the threads have is put together as (count, mean, squared deviations).
-template <typename T, int V, bool RING>
+template <typename T, int V>
 __device__ __forceinline__ void gn_stats(const Shape& h, const Share& sh, const Place& pl, uint8_t* gn_raw, const T* x, float2* part) {
-  using Stream = Rows<T, V, 1, RING>;
+  using Stream = Rows<T, V, 1>;
   const int C = h.C, G = h.G;
   float2* gn_ent = reinterpret_cast<float2*>(gn_raw + Stream::BYTES);       // [rg][C]: mean and squared deviations of a row class, then [0][C] of the chunk
   const int span_rows = sh.r1 - sh.r0;
@@ -459,11 +462,11 @@ __device__ __forceinline__ void gn_stats(const Shape& h, const Share& sh, const 
   });
 }
 
-template <typename T, int V, bool RING>
+template <typename T, int V>
 __global__ void __launch_bounds__(GN_THREADS, gn_per_sm(false)) gn_stats_kernel(const Shape h, const T* x, float2* part) {
   extern __shared__ __align__(16) uint8_t gn_raw[];
   pdl_trigger();
-  gn_stats<T, V, RING>(h, share_of(h, blockIdx.x), place_of(h), gn_raw, x, part);
+  gn_stats<T, V>(h, share_of(h, blockIdx.x), place_of(h), gn_raw, x, part);
 }
 
 // floats of a per-channel array in shared memory: what follows it is 16-byte aligned again, whatever C is
@@ -539,10 +542,10 @@ __global__ void __launch_bounds__(GN_THREADS) gn_merge_kernel(const Shape h, con
 // shared: mean, rstd by group, then by channel -mean, A = rstd * gamma, beta; z = (x - mean) * A + beta
 struct GnApply { const void *gamma, *beta; float *mean, *rstd; int pdt, act; float eps; };
 // merge_chunks: how many of `part` there are a sample (one, of all rows, behind gn_merge_kernel)
-template <typename T, int V, bool DROP, bool RING, typename Wait>
+template <typename T, int V, bool DROP, typename Wait>
 __device__ __forceinline__ void gn_apply(const Shape& h, const Share& sh, const Place& pl, uint8_t* gn_raw, const T* x, const float2* part, int merge_chunks,
                                          T* y, const GnApply& q, const DropKey& key, Wait wait) {
-  using Stream = Rows<T, V, 1, RING>;
+  using Stream = Rows<T, V, 1>;
   const int C = h.C, G = h.G, cp = gn_pad(C);
   float* gn_c = reinterpret_cast<float*>(gn_raw + Stream::BYTES);
   float *c_mu = gn_c, *c_a = c_mu + cp, *c_b = c_a + cp;
@@ -578,27 +581,29 @@ __device__ __forceinline__ void gn_apply(const Shape& h, const Share& sh, const 
   for (int col = pl.col; col < pl.cols; col += GN_THREADS) {
     const Nums<V> mu = take_v<V>(c_mu, col), A = take_v<V>(c_a, col), Bt = take_v<V>(c_b, col);
     if (col != pl.col) n = gn_begin(in, gn_raw, h, sh, pl, V, col);
-    uint32_t i = static_cast<uint32_t>(pl.row) * h.allC + col * V;
+    with_activation(q.act, [&](auto activation) {
+      uint32_t i = static_cast<uint32_t>(pl.row) * h.allC + col * V;
 #pragma unroll 2
-    for (int r = 0; r < n; ++r, i += in.stride) {
-      Nums<V> f[1];
-      in.take(f);
-      const Nums<V> d = f[0] + mu;
-      in.advance();
-      Nums<V> a = activate<V>(q.act, n_fma<V>(d, A, Bt));
-      if (DROP) a = n_drop<V>(key, step, start + i, a);
-      store_v<T, V>(out + i, a);
-    }
+      for (int r = 0; r < n; ++r, i += in.stride) {
+        Nums<V> f[1];
+        in.take(f);
+        const Nums<V> d = f[0] + mu;
+        in.advance();
+        Nums<V> a = activate<decltype(activation)::value, V>(n_fma<V>(d, A, Bt));
+        if (DROP) a = n_drop<V>(key, step, start + i, a);
+        store_v<T, V>(out + i, a);
+      }
+    });
   }
 }
 
-template <typename T, int V, bool DROP, bool RING>
+template <typename T, int V, bool DROP>
 __global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_apply_kernel(const Shape h, const T* x, const float2* part, int merge_chunks, T* y, const GnApply q,
                                                                  const DropKey key) {
   extern __shared__ __align__(16) uint8_t gn_raw[];
   pdl_trigger();
   // from the back: what the first pass read last is in L2
-  gn_apply<T, V, DROP, RING>(h, share_of(h, gridDim.x - 1 - blockIdx.x), place_of(h), gn_raw, x, part, merge_chunks, y, q, key, [] { pdl_wait(); });
+  gn_apply<T, V, DROP>(h, share_of(h, gridDim.x - 1 - blockIdx.x), place_of(h), gn_raw, x, part, merge_chunks, y, q, key, [] { pdl_wait(); });
 }
 
 // ---- both passes in one kernel --------------------------------------------------------------------------
@@ -612,13 +617,13 @@ __device__ __forceinline__ Share cluster_share(const Shape& h) {
   const int slabs = h.allG / h.G, id = quotient(blockIdx.x, h.chunks, h.by_chunks);
   return share_of(h, id / slabs, id % slabs, blockIdx.x - id * h.chunks);
 }
-template <typename T, int V, bool DROP, bool RING>
+template <typename T, int V, bool DROP>
 __global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_fwd_cluster_kernel(const Shape h, const T* x, float2* part, T* y, const GnApply q, const DropKey key) {
   extern __shared__ __align__(16) uint8_t gn_raw[];
   const Share sh = cluster_share(h);
   const Place pl = place_of(h);
-  gn_stats<T, V, RING>(h, sh, pl, gn_raw, x, part);
-  gn_apply<T, V, DROP, RING>(h, sh, pl, gn_raw, x, part, h.chunks, y, q, key, [] { cluster_meet(); });
+  gn_stats<T, V>(h, sh, pl, gn_raw, x, part);
+  gn_apply<T, V, DROP>(h, sh, pl, gn_raw, x, part, h.chunks, y, q, key, [] { cluster_meet(); });
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------
@@ -635,20 +640,20 @@ __device__ __forceinline__ void bwd_constants(float* c_mu, float* c_a, float* c_
   }
 }
 // f[0] = dy becomes gz, f[1] = x becomes x - mean, for V elements at flat index i
-template <int V, bool DROP>
-__device__ __forceinline__ void gz_dev(Nums<V> f[2], size_t i, const Nums<V>& mu, const Nums<V>& A, const Nums<V>& Bt, int act, const DropKey& key,
+template <int ACT, int V, bool DROP>
+__device__ __forceinline__ void gz_dev(Nums<V> f[2], size_t i, const Nums<V>& mu, const Nums<V>& A, const Nums<V>& Bt, const DropKey& key,
                                        uint32_t step) {
   f[1] = f[1] + mu;
   if (DROP) f[0] = n_drop<V>(key, step, i, f[0]);
-  if (act != FDP_ACT_NONE) f[0] = times_slope<V>(act, n_fma<V>(f[1], A, Bt), f[0]);
+  if (ACT != FDP_ACT_NONE) f[0] = times_slope<ACT, V>(n_fma<V>(f[1], A, Bt), f[0]);
 }
 
 // first pass: part[0][b][chunk][c] = sum gz * xhat, part[1] = sum gz; gpart[b][chunk][g] = (sum_c gamma * sum gz, the same with xhat)
 struct GnBwd { const void *gamma, *beta; const float *mean, *rstd; int pdt, act; };
-template <typename T, int V, bool DROP, bool RING>
+template <typename T, int V, bool DROP>
 __device__ __forceinline__ void gn_bwd_sums(const Shape& h, const Share& sh, const Place& pl, uint8_t* gn_raw, const T* dy, const T* x, const GnBwd& q,
                                             float* part, float2* gpart, const DropKey& key) {
-  using Stream = Rows<T, V, 2, RING>;
+  using Stream = Rows<T, V, 2>;
   const int C = h.C, G = h.G, cp = gn_pad(C), cg = h.cg;
   float* gn_c = reinterpret_cast<float*>(gn_raw + Stream::BYTES);
   float *c_mu = gn_c, *c_a = c_mu + cp, *c_b = c_a + cp;
@@ -668,16 +673,18 @@ __device__ __forceinline__ void gn_bwd_sums(const Shape& h, const Share& sh, con
     const Nums<V> mu = take_v<V>(c_mu, col), A = take_v<V>(c_a, col), Bt = take_v<V>(c_b, col);
     Nums<V> t1 = n_all<V>(0.f), t2 = t1;
     if (col != pl.col) n = gn_begin(in, gn_raw, h, sh, pl, V, col);
-    uint32_t i = static_cast<uint32_t>(pl.row) * h.allC + col * V;
+    with_activation(q.act, [&](auto activation) {
+      uint32_t i = static_cast<uint32_t>(pl.row) * h.allC + col * V;
 #pragma unroll 2
-    for (int r = 0; r < n; ++r, i += in.stride) {
-      Nums<V> f[2];
-      in.take(f);
-      gz_dev<V, DROP>(f, start + i, mu, A, Bt, q.act, key, step);
-      in.advance();
-      t1 = t1 + f[0];
-      t2 = n_fma<V>(f[0], f[1], t2);
-    }
+      for (int r = 0; r < n; ++r, i += in.stride) {
+        Nums<V> f[2];
+        in.take(f);
+        gz_dev<decltype(activation)::value, V, DROP>(f, start + i, mu, A, Bt, key, step);
+        in.advance();
+        t1 = t1 + f[0];
+        t2 = n_fma<V>(f[0], f[1], t2);
+      }
+    });
     n_get<V>(t1, s1);
     n_get<V>(t2, s2);
     if (apart) {
@@ -717,12 +724,12 @@ __device__ __forceinline__ void gn_bwd_sums(const Shape& h, const Share& sh, con
     if (valid && k == 0) gpart[(static_cast<size_t>(sh.b) * h.chunks + sh.chunk) * h.allG + sh.g0 + g] = make_float2(u, v);
   });
 }
-template <typename T, int V, bool DROP, bool RING>
+template <typename T, int V, bool DROP>
 __global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_bwd_sums_kernel(const Shape h, const T* dy, const T* x, const GnBwd q, float* part, float2* gpart,
                                                                                const DropKey key) {
   extern __shared__ __align__(16) uint8_t gn_raw[];
   pdl_trigger();
-  gn_bwd_sums<T, V, DROP, RING>(h, share_of(h, blockIdx.x), place_of(h), gn_raw, dy, x, q, part, gpart, key);
+  gn_bwd_sums<T, V, DROP>(h, share_of(h, blockIdx.x), place_of(h), gn_raw, dy, x, q, part, gpart, key);
 }
 
 // per-sample gradients from their chunks: out[tensor][b][c], and the sums of squares of every 32 columns, one block's
@@ -752,10 +759,10 @@ __global__ void __launch_bounds__(GN_THREADS) gn_psgrad_kernel(const float* part
   gn_psgrad(blockIdx.x, red, part, out, sumsq, chunks, C);
 }
 // second pass: dx = A * gz - c1 - (x - mean) * c2, c1 = rstd * s1, c2 = rstd^2 * s2
-template <typename T, int V, bool DROP, bool RING, typename Wait>
+template <typename T, int V, bool DROP, typename Wait>
 __device__ __forceinline__ void gn_bwd_dx(const Shape& h, const Share& sh, const Place& pl, uint8_t* gn_raw, const T* dy, const T* x, const GnBwd& q,
                                           const float2* gpart, int merge_chunks, T* dx, const DropKey& key, Wait wait) {
-  using Stream = Rows<T, V, 2, RING>;
+  using Stream = Rows<T, V, 2>;
   const int C = h.C, G = h.G, cp = gn_pad(C), cg = h.cg;
   float* gn_c = reinterpret_cast<float*>(gn_raw + Stream::BYTES);
   float *c_mu = gn_c, *c_a = c_mu + cp, *c_b = c_a + cp, *c_1 = c_b + cp, *c_2 = c_1 + cp;
@@ -782,21 +789,23 @@ __device__ __forceinline__ void gn_bwd_dx(const Shape& h, const Share& sh, const
   for (int col = pl.col; col < pl.cols; col += GN_THREADS) {
     const Nums<V> mu = take_v<V>(c_mu, col), A = take_v<V>(c_a, col), Bt = take_v<V>(c_b, col), k1 = take_v<V>(c_1, col), k2 = take_v<V>(c_2, col);
     if (col != pl.col) n = gn_begin(in, gn_raw, h, sh, pl, V, col);
-    uint32_t i = static_cast<uint32_t>(pl.row) * h.allC + col * V;
+    with_activation(q.act, [&](auto activation) {
+      uint32_t i = static_cast<uint32_t>(pl.row) * h.allC + col * V;
 #pragma unroll 2
-    for (int r = 0; r < n; ++r, i += in.stride) {
-      Nums<V> f[2];
-      in.take(f);
-      gz_dev<V, DROP>(f, start + i, mu, A, Bt, q.act, key, step);
-      in.advance();
-      store_v<T, V>(out + i, n_fma<V>(f[0], A, n_fma<V>(f[1], k2, k1)));
-    }
+      for (int r = 0; r < n; ++r, i += in.stride) {
+        Nums<V> f[2];
+        in.take(f);
+        gz_dev<decltype(activation)::value, V, DROP>(f, start + i, mu, A, Bt, key, step);
+        in.advance();
+        store_v<T, V>(out + i, n_fma<V>(f[0], A, n_fma<V>(f[1], k2, k1)));
+      }
+    });
   }
 }
 
 // The launch has blocks in front that form the per-sample gradients, which need the first pass only: no launch of their own.
 struct GnPsgrad { int pieces; const float* part; float *out, *sumsq; };
-template <typename T, int V, bool DROP, bool RING>
+template <typename T, int V, bool DROP>
 __global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_bwd_dx_kernel(const Shape h, const T* dy, const T* x, const GnBwd q, const float2* gpart,
                                                                              int merge_chunks, T* dx, const GnPsgrad ps, const DropKey key) {
   extern __shared__ __align__(16) uint8_t gn_raw[];
@@ -806,18 +815,18 @@ __global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_bwd_dx_kernel(
     gn_psgrad(blockIdx.x, reinterpret_cast<float*>(gn_raw), ps.part, ps.out, ps.sumsq, h.chunks, h.C);
     return;
   }
-  gn_bwd_dx<T, V, DROP, RING>(h, share_of(h, gridDim.x - 1 - blockIdx.x), place_of(h), gn_raw, dy, x, q, gpart, merge_chunks, dx, key,
+  gn_bwd_dx<T, V, DROP>(h, share_of(h, gridDim.x - 1 - blockIdx.x), place_of(h), gn_raw, dy, x, q, gpart, merge_chunks, dx, key,
                               [] { pdl_wait(); });
 }
 // In a cluster every block also forms its part of the sample's gradients: one of h.chunks stretches of the channels.
-template <typename T, int V, bool DROP, bool RING>
+template <typename T, int V, bool DROP>
 __global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_bwd_cluster_kernel(const Shape h, const T* dy, const T* x, const GnBwd q, float* part,
                                                                                   float2* gpart, T* dx, const GnPsgrad ps, const DropKey key) {
   extern __shared__ __align__(16) uint8_t gn_raw[];
   const Share sh = cluster_share(h);
   const Place pl = place_of(h);
   pdl_trigger();
-  gn_bwd_sums<T, V, DROP, RING>(h, sh, pl, gn_raw, dy, x, q, part, gpart, key);
+  gn_bwd_sums<T, V, DROP>(h, sh, pl, gn_raw, dy, x, q, part, gpart, key);
   __syncthreads();
   auto gradients = [&] {
     cluster_meet();
@@ -843,7 +852,7 @@ __global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_bwd_cluster_ke
       if (threadIdx.x == 0) ps.sumsq[(static_cast<size_t>(t) * h.B + sh.b) * parts + at] = v;
     }
   };
-  if (dx != nullptr) gn_bwd_dx<T, V, DROP, RING>(h, sh, pl, gn_raw, dy, x, q, gpart, h.chunks, dx, key, gradients);
+  if (dx != nullptr) gn_bwd_dx<T, V, DROP>(h, sh, pl, gn_raw, dy, x, q, gpart, h.chunks, dx, key, gradients);
   else gradients();
 }
 
@@ -885,11 +894,9 @@ __global__ void __launch_bounds__(GN_THREADS) gn_clip_kernel(const float* psgrad
   }
 }
 
-// Rows of up to GN_RING_CHANNELS channels leave room for the ring beside their constants (five floats a channel and two
-// a group); longer ones are loaded into registers.
-constexpr int GN_RING_CHANNELS = 4096;
-constexpr size_t GN_SMEM_MOST = GN_MAX_CHANNELS * 24;
-static_assert(GN_SMEM_MOST <= 227 * 1024 && GN_RING_CHANNELS * 20 + 3 * 16384 <= GN_SMEM_MOST, "shared memory of a block");
+// constants of GN_MAX_CHANNELS channels (five floats, or three and two sums) beside a ring of 32 KB
+constexpr size_t GN_SMEM_MOST = GN_MAX_CHANNELS * 20 + 32768;
+static_assert(GN_SMEM_MOST <= 227 * 1024 && Rows<float, 4, 2>::BYTES <= 32768 && Rows<__half, 8, 2>::BYTES <= 32768, "shared memory of a block");
 template <auto KERNEL>
 bool opt_in(size_t bytes) {
   static bool done[64];
@@ -946,9 +953,9 @@ Shape shape_of(const GnArgs& a, const GnPlan& pl, int V) {
   return h;
 }
 
-template <typename T, int V, bool DROP, bool RING>
+template <typename T, int V, bool DROP>
 int fwd_typed(const GnArgs& a, const GnPlan& pl, cudaStream_t s) {
-  constexpr size_t ring = Rows<T, V, 1, RING>::BYTES;
+  constexpr size_t ring = Rows<T, V, 1>::BYTES;
   const Shape h = shape_of(a, pl, V);
   const size_t ent = ring + sizeof(float2) * static_cast<size_t>(rows_at_a_time(h.C / V)) * h.C;
   const size_t con = ring + sizeof(float) * (3 * gn_pad(h.C) + 2 * h.G);
@@ -958,19 +965,19 @@ int fwd_typed(const GnArgs& a, const GnPlan& pl, cudaStream_t s) {
   const unsigned grid = static_cast<unsigned>(static_cast<size_t>(a.B) * pl.slabs * pl.chunks);
   const T* x = static_cast<const T*>(a.x);
   T* y = static_cast<T*>(a.y);
-  if (pl.cluster) return gn_launch_clusters<gn_fwd_cluster_kernel<T, V, DROP, RING>>(grid, pl.chunks, ent > con ? ent : con, s, h, x, part, y, q, key);
+  if (pl.cluster) return gn_launch_clusters<gn_fwd_cluster_kernel<T, V, DROP>>(grid, pl.chunks, ent > con ? ent : con, s, h, x, part, y, q, key);
   const bool merge = pl.chunks > GN_MERGE_CHUNKS;
-  int st = gn_launch<gn_stats_kernel<T, V, RING>>(grid, ent, false, s, h, x, part);
+  int st = gn_launch<gn_stats_kernel<T, V>>(grid, ent, false, s, h, x, part);
   if (st == FDP_OK && merge) st = gn_launch<gn_merge_kernel<true>>(a.B, 0, true, s, h, static_cast<const float2*>(part), whole);
   if (st == FDP_OK)
-    st = gn_launch<gn_apply_kernel<T, V, DROP, RING>>(grid, con, true, s, h, x, static_cast<const float2*>(merge ? whole : part), merge ? 1 : pl.chunks, y, q, key);
+    st = gn_launch<gn_apply_kernel<T, V, DROP>>(grid, con, true, s, h, x, static_cast<const float2*>(merge ? whole : part), merge ? 1 : pl.chunks, y, q, key);
   return st;
 }
 
 // nparts: sums of squares a sample
-template <typename T, int V, bool DROP, bool RING>
+template <typename T, int V, bool DROP>
 int bwd_typed(const GnArgs& a, const GnPlan& pl, bool need_dw, int* nparts, cudaStream_t s) {
-  constexpr size_t ring = Rows<T, V, 2, RING>::BYTES;
+  constexpr size_t ring = Rows<T, V, 2>::BYTES;
   const Shape h = shape_of(a, pl, V);
   const size_t con = sizeof(float) * 3 * gn_pad(h.C), ent = sizeof(float2) * static_cast<size_t>(rows_at_a_time(h.C / V)) * h.C;
   const size_t sums = ring + (h.C / V > GN_THREADS ? con + sizeof(float2) * h.C : ent > con ? ent : con);
@@ -985,18 +992,18 @@ int bwd_typed(const GnArgs& a, const GnPlan& pl, bool need_dw, int* nparts, cuda
   GnPsgrad ps{0, a.part, need_dw ? a.psgrad : nullptr, a.sumsq};
   if (pl.cluster) {
     *nparts = pl.slabs * pl.chunks;
-    return gn_launch_clusters<gn_bwd_cluster_kernel<T, V, DROP, RING>>(grid, pl.chunks, sums > out ? sums : out, s, h, dy, x, q, a.part,
+    return gn_launch_clusters<gn_bwd_cluster_kernel<T, V, DROP>>(grid, pl.chunks, sums > out ? sums : out, s, h, dy, x, q, a.part,
                                                                        dx != nullptr ? gpart : nullptr, dx, ps, key);
   }
   *nparts = ceil_div(a.C, 32);
   const bool merge = pl.chunks > GN_MERGE_CHUNKS;
   const int pieces = need_dw ? 2 * a.B * *nparts : 0;
-  int st = gn_launch<gn_bwd_sums_kernel<T, V, DROP, RING>>(grid, sums, false, s, h, dy, x, q, a.part, dx != nullptr ? gpart : nullptr, key);
+  int st = gn_launch<gn_bwd_sums_kernel<T, V, DROP>>(grid, sums, false, s, h, dy, x, q, a.part, dx != nullptr ? gpart : nullptr, key);
   if (st == FDP_OK && dx != nullptr) {
     if (merge) st = gn_launch<gn_merge_kernel<false>>(a.B, 0, true, s, h, static_cast<const float2*>(gpart), whole);
     ps.pieces = pieces;
     if (st == FDP_OK)
-      st = gn_launch<gn_bwd_dx_kernel<T, V, DROP, RING>>(grid + pieces, out, true, s, h, dy, x, q, static_cast<const float2*>(merge ? whole : gpart),
+      st = gn_launch<gn_bwd_dx_kernel<T, V, DROP>>(grid + pieces, out, true, s, h, dy, x, q, static_cast<const float2*>(merge ? whole : gpart),
                                                          merge ? 1 : pl.chunks, dx, ps, key);
   } else if (st == FDP_OK && need_dw) {
     st = gn_launch<gn_psgrad_kernel>(pieces, 0, true, s, static_cast<const float*>(a.part), a.psgrad, a.sumsq, pl.chunks, a.C);
@@ -1008,19 +1015,19 @@ template <typename T, bool DROP>
 int fwd_any(const GnArgs& a, const GnPlan& pl, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const bool aligned = aligned16(a.x) && aligned16(a.y);
-  if (pl.vec == V && aligned) return a.C / pl.slabs <= GN_RING_CHANNELS ? fwd_typed<T, V, DROP, true>(a, pl, s) : fwd_typed<T, V, DROP, false>(a, pl, s);
+  if (pl.vec == V && aligned) return fwd_typed<T, V, DROP>(a, pl, s);
   if constexpr (V == 8)
-    if (pl.vec == 2 && aligned && a.C / pl.slabs <= GN_RING_CHANNELS) return fwd_typed<T, 2, DROP, true>(a, pl, s);
-  return fwd_typed<T, 1, DROP, false>(a, pl, s);
+    if (pl.vec == 2 && aligned) return fwd_typed<T, 2, DROP>(a, pl, s);
+  return fwd_typed<T, 1, DROP>(a, pl, s);
 }
 template <typename T, bool DROP>
 int bwd_any(const GnArgs& a, const GnPlan& pl, bool need_dw, int* nparts, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const bool aligned = aligned16(a.x) && aligned16(a.dy) && (a.dx == nullptr || aligned16(a.dx));
-  if (pl.vec == V && aligned) return a.C / pl.slabs <= GN_RING_CHANNELS ? bwd_typed<T, V, DROP, true>(a, pl, need_dw, nparts, s) : bwd_typed<T, V, DROP, false>(a, pl, need_dw, nparts, s);
+  if (pl.vec == V && aligned) return bwd_typed<T, V, DROP>(a, pl, need_dw, nparts, s);
   if constexpr (V == 8)
-    if (pl.vec == 2 && aligned && a.C / pl.slabs <= GN_RING_CHANNELS) return bwd_typed<T, 2, DROP, true>(a, pl, need_dw, nparts, s);
-  return bwd_typed<T, 1, DROP, false>(a, pl, need_dw, nparts, s);
+    if (pl.vec == 2 && aligned) return bwd_typed<T, 2, DROP>(a, pl, need_dw, nparts, s);
+  return bwd_typed<T, 1, DROP>(a, pl, need_dw, nparts, s);
 }
 template <typename T>
 int fwd_drop(const GnArgs& a, const GnPlan& pl, cudaStream_t s) { return a.drop != nullptr ? fwd_any<T, true>(a, pl, s) : fwd_any<T, false>(a, pl, s); }
