@@ -54,23 +54,18 @@ __device__ __forceinline__ void drop_philox(const DropKey& k, uint32_t step, uin
   r[0] = c0; r[1] = c1; r[2] = c2; r[3] = c3;
 }
 
-// A group's 16-bit numbers, two a word, after the border has been settled: number e is kept if it is above the upper half of
-// `bound`.  A comparison and a selection an element; collected into a mask of bits and taken apart again, the eight elements of
-// a group took 161 instructions with everything, now 105 (134 M elements bf16: 142 us, the integer pipe full, now 92).
+// A group's 16-bit numbers, two a word, after the border has been settled: number e is kept if it is at least the half of
+// `bound` that it faces.
 struct Draw { uint32_t w[4], bound; };
 __device__ __forceinline__ Draw draw8(const DropKey& k, uint32_t step, uint64_t group) {
   group += k.offset;
   Draw d;
   drop_philox(k, step, group, d.w);
-  d.bound = (k.hi << 16) | 0xFFFFu;
   const uint32_t both = k.hi | (k.hi << 16);
-  uint32_t tie = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t x = d.w[j] ^ both;                // a half that is zero has 16 bits like T's
-    tie |= (x - 0x00010001u) & ~x;                   // (a half above a zero half may report itself too: looked at again below)
-  }
-  if ((tie & 0x80008000u) != 0 || k.hi >= 65535u) {  // (from 65535 on no number is above the bound: settled one by one)
+  d.bound = both + 0x00010001u;
+  // a half of w ^ both that is zero has 16 bits like T's
+  const uint32_t m = __vminu2(__vminu2(d.w[0] ^ both, d.w[1] ^ both), __vminu2(d.w[2] ^ both, d.w[3] ^ both));
+  if (((m - 0x00010001u) & ~m & 0x80008000u) != 0 || k.hi >= 65535u) {  // (from 65535 on no number is above T's 16 bits: settled one by one)
     uint32_t q[4];
     drop_philox(k, step, group | (1ull << 63), q);
 #pragma unroll
@@ -79,10 +74,11 @@ __device__ __forceinline__ Draw draw8(const DropKey& k, uint32_t step, uint64_t 
       const bool kl = l > k.hi || (l == k.hi && (q[j] & 0xFFFFu) >= k.lo), kh = h > k.hi || (h == k.hi && (q[j] >> 16) >= k.lo);
       d.w[j] = (kl ? 0xFFFFu : 0u) | (kh ? 0xFFFF0000u : 0u);
     }
-    d.bound = 0x7FFFFFFFu;
+    d.bound = 0x80008000u;
   }
   return d;
 }
+__device__ __forceinline__ bool draw_keeps(uint32_t word, uint32_t bound, int half) { return (half ? word >> 16 : word & 0xFFFFu) >= (bound & 0xFFFFu); }
 // a * b of pairs, as one instruction
 __device__ __forceinline__ void drop_scale2(float& a, float& b, float s) {
   asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(a), "+f"(b) : "f"(s));
@@ -93,7 +89,7 @@ __device__ __forceinline__ void drop_v(const DropKey& k, uint32_t step, uint64_t
   const Draw d = draw8(k, step, element >> 3);
   if constexpr (V == 1) {
     const uint32_t j = (element >> 1) & 3, w = j == 0 ? d.w[0] : j == 1 ? d.w[1] : j == 2 ? d.w[2] : d.w[3];
-    f[0] = (element & 1 ? w : w << 16) > d.bound ? f[0] * k.scale : 0.f;
+    f[0] = draw_keeps(w, d.bound, element & 1) ? f[0] * k.scale : 0.f;
   } else {
     uint32_t w[V / 2];
     if constexpr (V == 8) {
@@ -110,8 +106,8 @@ __device__ __forceinline__ void drop_v(const DropKey& k, uint32_t step, uint64_t
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) {
       drop_scale2(f[2 * j], f[2 * j + 1], k.scale);
-      f[2 * j] = (w[j] << 16) > d.bound ? f[2 * j] : 0.f;
-      f[2 * j + 1] = w[j] > d.bound ? f[2 * j + 1] : 0.f;
+      f[2 * j] = (w[j] << 16) >= (d.bound << 16) ? f[2 * j] : 0.f;
+      f[2 * j + 1] = w[j] >= (d.bound & 0xFFFF0000u) ? f[2 * j + 1] : 0.f;
     }
   }
 }
