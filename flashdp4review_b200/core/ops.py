@@ -445,24 +445,29 @@ class DropoutSpec:
     step_device: object = None    # a one-element int32 CUDA tensor the kernels add to `step` when they run
 
 
-def _drop(spec):
+def _drop(spec, device=None):
     if spec is None:
         return None
+    counter = spec.step_device
+    if counter is not None and (counter.dtype != torch.int32 or counter.numel() != 1 or not counter.is_cuda
+                                or (device is not None and counter.device != device)):
+        raise ValueError(f"dropout's step counter has to be one int32 on the input's GPU, but got {tuple(counter.shape)} "
+                         f"of {counter.dtype} on {counter.device}")
     if not 0.0 <= spec.p <= 1.0:
         raise ValueError(f"dropout probability has to be between 0 and 1, but got {spec.p}")
     if not 0 <= spec.offset < 1 << 60:
         raise ValueError(f"dropout offset has to be between 0 and 2^60, but got {spec.offset}")
     return (float(spec.p), int(spec.seed) & (2 ** 64 - 1), int(spec.offset), int(spec.stream_id) & 0xFFFFFFFF,
-            int(spec.step) & 0xFFFFFFFF, spec.step_device.data_ptr() if spec.step_device is not None else None)
+            int(spec.step) & 0xFFFFFFFF, None if counter is None else counter.data_ptr())
 
 
 def dropout(input, spec, residual=None, out=None):
     """Dropout of `input` (plus `residual`, of the input's shape and dtype) under the mask of `spec`, elements numbered in
     row-major order.  A dropped element is 0 whatever it held.  `out`: a contiguous tensor to write into; it may be the
-    input or the residual."""
+    input or the residual, but not lie over a part of either."""
     host = _lib.host()
     _require_cuda(input, residual, out)
-    code, d = _dt(input.dtype), _drop(spec)
+    code, d = _dt(input.dtype), _drop(spec, input.device)
     if residual is not None and (residual.shape != input.shape or residual.dtype != input.dtype):
         raise RuntimeError(f"residual must be a {tuple(input.shape)} tensor of {input.dtype}, "
                            f"got {tuple(residual.shape)} of {residual.dtype}")
@@ -514,7 +519,7 @@ def group_norm_forward(input, weight, bias, num_groups, eps=1e-5, *, activation=
     "silu", "gelu" or "gelu_tanh"; `dropout`: a DropoutSpec, whose mask is that of `dropout(y, spec)`."""
     host = _lib.host()
     _require_cuda(input, weight, bias)
-    act, spec, code = _activation(activation), _drop(dropout), _dt(input.dtype)
+    act, spec, code = _activation(activation), _drop(dropout, input.device), _dt(input.dtype)
     x = input.contiguous()
     T, w, b, pdt = _group_norm_args(x, weight, bias, num_groups)
     st, y, mean, rstd = host.group_norm_fwd(x, w, b, T, num_groups, float(eps), act, code, pdt, spec)
@@ -529,7 +534,7 @@ def dp_group_norm_backward(grad_output, input, weight, bias, mean, rstd, num_gro
     in the place of what is not needed; with return_norms the per-sample norms of both follow."""
     host = _lib.host()
     _require_cuda(grad_output, input, weight, bias, mean, rstd)
-    act, spec, code = _activation(activation), _drop(dropout), _dt(input.dtype)
+    act, spec, code = _activation(activation), _drop(dropout, input.device), _dt(input.dtype)
     x, dy = input.contiguous(), grad_output.to(input.dtype).contiguous()
     T, w, b, pdt = _group_norm_args(x, weight, bias, num_groups)
     need_dw = need_dw and w is not None

@@ -115,7 +115,9 @@ int check_dropout(const fdp_dropout_params* p) {
 int check_group_norm(int B, int T, int C, int G, int activation, int dtype, int param_dtype, const fdp_dropout_params* drop) {
   if (B <= 0 || T <= 0 || C <= 0 || G <= 0 || activation < FDP_ACT_NONE || activation > FDP_ACT_GELU_TANH) return FDP_ERR_ARG;
   if (!valid_dtype(dtype) || !valid_dtype(param_dtype)) return FDP_ERR_DTYPE;
-  if (C % G != 0 || C > GN_MAX_CHANNELS || static_cast<long long>(B) * T >= (1ll << 31) / 2) return FDP_ERR_SHAPE;
+  // (blocks of a launch are numbered in 31 bits: a chunk of a sample each, and one for 32 channels of each of its two gradients)
+  if (C % G != 0 || C > GN_MAX_CHANNELS || static_cast<long long>(B) * T >= (1ll << 31) / 2 || static_cast<long long>(B) * ceil_div(C, 32) >= (1ll << 31) / 4)
+    return FDP_ERR_SHAPE;
   return check_dropout(drop);
 }
 // workspace of fdp_fp8_matmul: quantised x, its exponents, the parts of a K split
@@ -856,6 +858,11 @@ int fdp_dropout(const void* x, const void* residual, void* y, size_t n, int dtyp
   if (st != FDP_OK) return st;
   if (n == 0) return FDP_OK;
   if (x == nullptr || y == nullptr) return FDP_ERR_ARG;
+  // y is one of the others or apart from both: in part over them, it would be written before they are read
+  const size_t bytes = n * dtype_size(dtype);
+  for (const void* in : {x, residual})
+    if (in != nullptr && in != y && static_cast<const char*>(in) < static_cast<const char*>(y) + bytes && static_cast<const char*>(y) < static_cast<const char*>(in) + bytes)
+      return FDP_ERR_ARG;
   if ((st = current_device_ok()) != FDP_OK) return st;
   dropout(x, residual, y, n, dtype, p, static_cast<cudaStream_t>(stream));
   FDP_LAUNCH_OK();

@@ -1061,7 +1061,8 @@ GnPlan gn_plan(int B, int T, int C, int G, int element, int tensors, bool drop) 
     for (int d = 1; d <= G; ++d) {
       if (G % d != 0) continue;
       const int cs = C / d;
-      if (cs % pl.vec != 0 || (d > 1 && cs * element < SEGMENT)) continue;
+      if (d > 1 && cs * element < SEGMENT) break;
+      if (cs % pl.vec != 0) continue;
       const int most = ceil_div(T, 2 * rows_at_a_time(cs / pl.vec));            // chunks of at least two rows a thread
       int k = 1;
       while (k < 16 && 2 * k <= most && (sample / d / k > PIECE || static_cast<long long>(B) * d * k < GN_WAVE)) k *= 2;

@@ -99,6 +99,11 @@ void refuse(const char* what, const Tensor& t) {
   s += ") on " + std::string(c10::DeviceTypeName(t.device().type(), true)) + (t.device().has_index() ? ":" + std::to_string(t.device().index()) : "");
   throw std::runtime_error(s);
 }
+// a size that the entry points take in 32 bits
+int size32(int64_t n, const char* what, const Tensor& t) {
+  if (n > INT32_MAX) refuse(what, t);
+  return static_cast<int>(n);
+}
 // weight of a product that contracts `k` columns: [n, k] or, with k_rows, [k, n] (n < 0: any)
 void check_weight(const Tensor& W, int64_t k, int64_t n, bool k_rows, const Tensor& like) {
   if (W.dim() != 2 || W.size(k_rows ? 0 : 1) != k || (n >= 0 && W.size(k_rows ? 1 : 0) != n)) refuse("weight does not fit the other operands", W);
@@ -349,7 +354,7 @@ py::tuple dropout(const Tensor& x, const OptTensor& residual, const OptTensor& o
 
 // parameters (both or neither) and statistics of a group norm over x [B, ..., C]
 void check_group_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, const OptTensor& mean, const OptTensor& rstd, const OptTensor& dy, int64_t G) {
-  const int64_t C = x.size(-1), B = x.size(0);
+  const int64_t C = size32(x.size(-1), "group norm: too many channels", x), B = size32(x.size(0), "group norm: too many samples", x);
   for (const OptTensor& t : {w, b})
     if (t.has_value() && (t->device() != x.device() || t->numel() != C)) refuse("group norm: parameters do not fit the input's channels", *t);
   for (const OptTensor& t : {mean, rstd})
@@ -402,22 +407,22 @@ Tensor fp8_matrix(const Tensor& like, int64_t rows, int64_t cols) {
 }
 // x [rows, cols] -> 8-bit numbers, scales [column blocks, rows]
 py::tuple fp8_quantize(const Tensor& x, int dt) {
+  const int rows = size32(x.size(0), "too many rows", x), cols = size32(x.size(1), "too many columns", x);
   const c10::cuda::CUDAGuard guard(x.device());
-  const int64_t rows = x.size(0), cols = x.size(1);
-  const Tensor q = fp8_matrix(x, rows, cols), scales = new_tensor(x, {(cols + 127) / 128, rows}, at::kFloat);
+  const Tensor q = fp8_matrix(x, rows, cols), scales = new_tensor(x, {(static_cast<int64_t>(cols) + 127) / 128, rows}, at::kFloat);
   int st;
   {
     py::gil_scoped_release nogil;
-    st = abi.fp8_quantize(ptr(x), ptr(q), static_cast<float*>(ptr(scales)), static_cast<int>(rows), static_cast<int>(cols), dt, stream(x));
+    st = abi.fp8_quantize(ptr(x), ptr(q), static_cast<float*>(ptr(scales)), rows, cols, dt, stream(x));
   }
   return py::make_tuple(st, q, scales);
 }
 py::tuple fp8_quantize_weight(const Tensor& w, int dt) {
+  const int r = size32(w.size(0), "too many rows", w), c = size32(w.size(1), "too many columns", w);
   const c10::cuda::CUDAGuard guard(w.device());
-  const int64_t rows = w.size(0), cols = w.size(1);
+  const int64_t rows = r, cols = c;
   const Tensor q = fp8_matrix(w, rows, cols), qt = fp8_matrix(w, cols, rows);
   const Tensor scales = new_tensor(w, {(rows + 127) / 128, (cols + 127) / 128}, at::kFloat);
-  const int r = static_cast<int>(rows), c = static_cast<int>(cols);
   const Tensor packed = new_tensor(w, {static_cast<int64_t>(abi.fp8_exponent_bytes(r, c))}, at::kByte);
   const Tensor packed_t = new_tensor(w, {static_cast<int64_t>(abi.fp8_exponent_bytes(c, r))}, at::kByte);
   int st;
@@ -429,11 +434,11 @@ py::tuple fp8_quantize_weight(const Tensor& w, int dt) {
 }
 // x (..., k) times w [n, k]^T in 8 bits
 py::tuple fp8_matmul(const Tensor& x, const Tensor& w, const Tensor& packed, const OptTensor& bias, int dt, int out_dt) {
-  const int64_t k = x.size(-1), n = w.size(0), rows = k > 0 ? x.numel() / k : 0;
+  const int64_t k = x.size(-1), n = w.size(0);
+  const int r = size32(k > 0 ? x.numel() / k : 0, "too many rows", x), nn = size32(n, "too many rows", w), kk = size32(k, "too many columns", x);
   if (w.device() != x.device() || packed.device() != x.device()) refuse("weight is on another device", w);
-  if (w.dim() != 2 || w.size(1) != k || w.scalar_type() != at::kFloat8_e4m3fn || w.stride(1) != 1 || w.stride(0) != abi.fp8_pitch(static_cast<int>(k)))
+  if (w.dim() != 2 || w.size(1) != k || w.scalar_type() != at::kFloat8_e4m3fn || w.stride(1) != 1 || w.stride(0) != abi.fp8_pitch(kk))
     refuse("weight does not fit the other operand", w);
-  const int r = static_cast<int>(rows), nn = static_cast<int>(n), kk = static_cast<int>(k);
   if (packed.scalar_type() != at::kByte || !packed.is_contiguous() || static_cast<size_t>(packed.numel()) != abi.fp8_exponent_bytes(nn, kk))
     refuse("exponents do not fit the weight", packed);
   if (bias.has_value() && (bias->numel() != n || bias->device() != x.device() || bias->scalar_type() != x.scalar_type())) refuse("bias does not fit the output's columns", *bias);

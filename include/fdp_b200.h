@@ -314,8 +314,8 @@ int fdp_layernorm_bwd_saturate(const void* dy, const void* x, const float* mean,
  * 0x44524F50; counter: group's low word, high word, stream_id, step) gives each number 16 bits, word i % 8 / 2, low half
  * first; the same 16 bits of the draw with bit 63 of the group set lie below them; the element is dropped if the 32 bits are
  * less than round(p 2^32).  p = 1 drops everything; a dropped element is 0 whatever x holds.
- * `offset`, in groups of eight and below 2^60, lets the ranks of a data-parallel job draw apart.  x, residual and y may be
- * one buffer.  n = 0 is a no-op.
+ * `offset`, in groups of eight and below 2^60, lets the ranks of a data-parallel job draw apart.  y may be x or residual,
+ * whole; over a part of either it is refused.  n = 0 is a no-op.
  */
 typedef struct fdp_dropout_params {
   double p;                    /* 0 <= p <= 1 */
@@ -331,8 +331,9 @@ int fdp_dropout(const void* x, const void* residual, void* y, size_t n, int dtyp
 /* ---- group norm, channels last, with activation and dropout behind it ---------------------------------
  * No counterpart in the reference.  Statistics are those of one sample, as per-sample clipping needs.
  *   x, y [B,T,C] in `dtype`; gamma, beta [C] in `param_dtype`, both or neither NULL (one and zero); mean, rstd float[B,G];
- *   C a multiple of G, at most 8192.  y = dropout(act(xhat * gamma + beta)), rounded once; drop NULL: no dropout (its
- *   elements are numbered as those of y).
+ *   C a multiple of G, at most 8192; B * T below 2^30 and B * ceil(C / 32) below 2^29.  y and dx are buffers of their own.
+ *   y = dropout(act(xhat * gamma + beta)), rounded once; drop NULL: no dropout (its elements are numbered as those
+ *   of y).
  * fdp_group_norm_bwd: dx as autograd's; dgamma / dbeta [C] in `param_dtype` are the per-sample gradients, each clipped by its
  *   norm, summed over the batch / batch_divisor, plus noise (param_id, param_id2), as in fdp_layernorm_bwd.  dx, the pair
  *   dgamma / dbeta and the norms (float[B]) may be NULL; beta is read where there is an activation.

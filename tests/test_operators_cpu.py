@@ -28,7 +28,7 @@ def test_gradient_against_differences():
 
 
 # ---- refusals: before anything is launched, so without a GPU -------------------------------------------------------------
-PTR, ODD = 4096, 4100          # not looked at by a call that is refused
+PTR, ODD = 8192, 8196          # not looked at by a call that is refused
 
 
 def _drop(p=0.1, offset=0):
@@ -41,17 +41,19 @@ def _dp(std=0.0):
 
 @pytest.mark.parametrize("change,status", [
     (dict(x=None), "ARG"), (dict(y=None), "ARG"), (dict(dtype=3), "DTYPE"), (dict(drop=None), "ARG"), (dict(drop=-0.1), "ARG"),
-    (dict(drop=1.1), "ARG"), (dict(drop=float("nan")), "ARG"), (dict(offset=1 << 60), "ARG"), (dict(n=0, x=None), "OK")])
+    (dict(drop=1.1), "ARG"), (dict(drop=float("nan")), "ARG"), (dict(offset=1 << 60), "ARG"), (dict(n=0, x=None), "OK"),
+    (dict(y=PTR + 16), "ARG"), (dict(y=PTR - 36), "ARG"), (dict(res=PTR + 4100, y=PTR + 4096), "ARG")])
 def test_dropout_entry_refuses(change, status):
-    a = dict(x=PTR, y=PTR, n=10, dtype=0, drop=0.1, offset=0, **{}) | change
+    a = dict(x=PTR, res=None, y=PTR, n=10, dtype=0, drop=0.1, offset=0) | change
     d = None if a["drop"] is None else _drop(a["drop"], a["offset"])
-    assert _lib.load().fdp_dropout(a["x"], None, a["y"], a["n"], a["dtype"], d, None) == getattr(_lib, "FDP_OK" if status == "OK" else "FDP_ERR_" + status)
+    assert _lib.load().fdp_dropout(a["x"], a["res"], a["y"], a["n"], a["dtype"], d, None) == getattr(_lib, "FDP_OK" if status == "OK" else "FDP_ERR_" + status)
 
 
 @pytest.mark.parametrize("change,status", [
     (dict(x=None), "ARG"), (dict(gamma=None), "ARG"), (dict(beta=None), "ARG"), (dict(mean=None), "ARG"), (dict(B=0), "ARG"), (dict(T=-1), "ARG"),
     (dict(C=0), "ARG"), (dict(G=0), "ARG"), (dict(act=5), "ARG"), (dict(act=-1), "ARG"), (dict(dtype=7), "DTYPE"), (dict(pdt=3), "DTYPE"),
-    (dict(G=3), "SHAPE"), (dict(C=8200, G=8), "SHAPE"), (dict(B=1 << 16, T=1 << 16), "SHAPE"), (dict(p=2.0), "ARG")])
+    (dict(G=3), "SHAPE"), (dict(C=8200, G=8), "SHAPE"), (dict(B=1 << 16, T=1 << 16), "SHAPE"), (dict(B=1 << 25, T=1, C=512), "SHAPE"),
+    (dict(p=2.0), "ARG")])
 def test_group_norm_entries_refuse(change, status):
     a = dict(x=PTR, gamma=PTR, beta=PTR, mean=PTR, B=2, T=4, C=16, G=4, act=0, dtype=0, pdt=0, p=0.1) | change
     want = getattr(_lib, "FDP_ERR_" + status)
@@ -109,6 +111,9 @@ def test_operators_refuse():
     for bad in (dict(p=-0.1), dict(p=1.5), dict(p=float("nan")), dict(offset=-1), dict(offset=1 << 60)):
         with pytest.raises(ValueError):
             ops._drop(core.DropoutSpec(**bad))
+    for counter in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64), torch.zeros(2, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="step counter"):
+            ops._drop(core.DropoutSpec(step_device=counter))
     with pytest.raises(ValueError, match="activation"):
         ops._activation("swish")
     for args in ((x, w, w, 3), (x, w, w, 0), (x, w, None, 4)):
@@ -117,6 +122,20 @@ def test_operators_refuse():
     for args in ((x[0, 0], w, w, 4), (x[:0], w, w, 4)):
         with pytest.raises(RuntimeError):
             ops._group_norm_args(*args)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """(not taken modulo 2^32, as a size that fits)"""
+    host, n = _lib.host(), (1 << 32) + 8
+    one = torch.zeros(1, 1)
+    w = torch.zeros(16, 16).to(torch.float8_e4m3fn)
+    for call in (lambda: host.fp8_quantize(one.expand(n, 16), 0), lambda: host.fp8_quantize(one.expand(4, n), 0),
+                 lambda: host.fp8_quantize_weight(one.expand(n, 16), 0), lambda: host.fp8_quantize_weight(one.expand(16, n), 0),
+                 lambda: host.fp8_matmul(one.expand(n, 16), w, torch.zeros(512, dtype=torch.uint8), None, 0, 0),
+                 lambda: host.group_norm_fwd(one.expand(2, n), None, None, 1, 8, 1e-5, 0, 0, 0, None),
+                 lambda: host.group_norm_fwd(one.expand(n, 8), None, None, 1, 8, 1e-5, 0, 0, 0, None)):
+        with pytest.raises(RuntimeError, match="too many"):
+            call()
 
 
 def test_products_in_8_bits_are_chosen_by_size():
