@@ -499,18 +499,21 @@ def _activation(name):
 
 def _group_norm_args(x, weight, bias, num_groups):
     """(T, contiguous weight, contiguous bias, parameter dtype code) of a group norm over x (B, ..., C)"""
-    if x.dim() < 2:
-        raise RuntimeError(f"group norm needs an input (B, ..., C), got {tuple(x.shape)}")
-    C = x.shape[-1]
+    shape = x.shape
+    if len(shape) < 2:
+        raise RuntimeError(f"group norm needs an input (B, ..., C), got {tuple(shape)}")
+    C, n = shape[-1], x.numel()
     if num_groups < 1 or C % num_groups != 0:
         raise ValueError(f"number of channels ({C}) must be divisible by num_groups ({num_groups})")
     if (weight is None) != (bias is None):
         raise ValueError("group norm has both a weight and a bias or neither")
-    if x.numel() == 0:
-        raise RuntimeError(f"group norm of an empty input {tuple(x.shape)}")
-    w = None if weight is None else weight.contiguous()
-    b = None if bias is None else bias.to(w.dtype).contiguous()
-    return x.numel() // (x.shape[0] * C), w, b, _lib.FDP_F32 if w is None else _dt(w.dtype)
+    if n == 0:
+        raise RuntimeError(f"group norm of an empty input {tuple(shape)}")
+    T = n // (shape[0] * C)
+    if weight is None:
+        return T, None, None, _lib.FDP_F32
+    dtype = weight.dtype
+    return T, weight.contiguous(), (bias if bias.dtype == dtype else bias.to(dtype)).contiguous(), _dt(dtype)
 
 
 def group_norm_forward(input, weight, bias, num_groups, eps=1e-5, *, activation=None, dropout=None):
@@ -535,7 +538,7 @@ def dp_group_norm_backward(grad_output, input, weight, bias, mean, rstd, num_gro
     host = _lib.host()
     _require_cuda(grad_output, input, weight, bias, mean, rstd)
     act, spec, code = _activation(activation), _drop(dropout, input.device), _dt(input.dtype)
-    x, dy = input.contiguous(), grad_output.to(input.dtype).contiguous()
+    x, dy = input.contiguous(), (grad_output if grad_output.dtype == input.dtype else grad_output.to(input.dtype)).contiguous()
     T, w, b, pdt = _group_norm_args(x, weight, bias, num_groups)
     need_dw = need_dw and w is not None
     if not (need_dx or need_dw):

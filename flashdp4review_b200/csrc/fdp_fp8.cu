@@ -103,7 +103,7 @@ __device__ __forceinline__ Eight<T> load_row8(const T* row, int col, int cols) {
 }
 
 // Rows: a half warp takes 128 columns of a row at a time, a block 16 rows x four blocks of columns: a row's four exponents are a
-// word of the unit described above.  HBM-bound: 5 bytes (16-bit) or 9 (fp32) of 2 or 4 read and 1 written.
+// word of the unit described above.  HBM-bound: 3 bytes an element of 16 bits (2 read, 1 written), 5 of 32.
 constexpr int QKB = 4;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) fp8_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, uint32_t* __restrict__ packed,
