@@ -713,18 +713,21 @@ void fp8_weight(const void* w, void* q, void* qt, float* scales, void* packed, v
 }
 
 // Pair tiles of 256 x 256, single CTAs' of 128 x 128, or those cut along K, whichever is expected to take least: a K block of
-// either tile takes about 0.27 us (the pair's is the tensor cores' time, the small tile's the time of its 32 KB from L2), a
-// tile 1.6 us beside them, the parts of a cut their way to L2 and back and a launch to add them up.
+// either tile takes about 0.27 us (the pair's is the tensor cores' time, the small tile's the time of its 32 KB from L2).  A
+// pair's tile takes 1.6 us beside them, a small one, whose store runs beside the next tile's products, 0.4; the pair starts and
+// ends half a microsecond slower (512 x 768 -> 768 bf16 with the quantisation 7.1 us in small tiles, 8.6 in pairs; 2048 x
+// 2048 -> 2048, where the small tiles take two rounds, 15.8 and 14.2).  The parts of a cut go to L2 and back and take a
+// launch to be added up.
 Fp8Plan fp8_plan(int M, int N, int K) {
-  constexpr double BLOCK = 0.27, TILE = 1.6, JOIN = 3.0, PARTS_BYTES_A_US = 5e6;
+  constexpr double BLOCK = 0.27, PAIR_TILE = 1.6, PAIR = 1.3, TILE = 0.4, ONE = 0.8, JOIN = 3.0, PARTS_BYTES_A_US = 5e6;
   const int kb = ceil_div(K, 128);
   const long long pairs = static_cast<long long>(ceil_div(M, 256)) * ceil_div(N, 256), tiles = static_cast<long long>(ceil_div(M, 128)) * ceil_div(N, 128);
   Fp8Plan pl{2, 256, 1, 0};
-  double best = static_cast<double>((pairs + 73) / 74) * (kb * BLOCK + TILE);
+  double best = static_cast<double>((pairs + 73) / 74) * (kb * BLOCK + PAIR_TILE) + PAIR;
   for (int split = 1; split <= 16 && split <= kb; split *= 2) {
     const double rows = M < 128 ? (M + 31) / 32 * 32 : 128;
     const double parts = split > 1 ? static_cast<double>(tiles) * split * rows * 128 * 4 : 0.0;
-    const double cost = static_cast<double>((tiles * split + 147) / 148) * (ceil_div(kb, split) * BLOCK + TILE) + (split > 1 ? JOIN + 2 * parts / PARTS_BYTES_A_US : 0.0);
+    const double cost = static_cast<double>((tiles * split + 147) / 148) * (ceil_div(kb, split) * BLOCK + TILE) + ONE + (split > 1 ? JOIN + 2 * parts / PARTS_BYTES_A_US : 0.0);
     if (cost < best) { best = cost; pl = Fp8Plan{1, 128, split, 0}; }
   }
   if (pl.split > 1) pl.parts_bytes = static_cast<size_t>(tiles) * pl.split * F8_BM * pl.bn * sizeof(float);

@@ -403,7 +403,9 @@ py::tuple group_norm_bwd(const Tensor& dy, const Tensor& x, const OptTensor& w, 
 
 // rows x pitch bytes, seen as rows x cols
 Tensor fp8_matrix(const Tensor& like, int64_t rows, int64_t cols) {
-  return new_tensor(like, {rows, abi.fp8_pitch(static_cast<int>(cols))}, at::kFloat8_e4m3fn).narrow(1, 0, cols);
+  const int64_t pitch = abi.fp8_pitch(static_cast<int>(cols));
+  const Tensor whole = new_tensor(like, {rows, pitch}, at::kFloat8_e4m3fn);
+  return pitch == cols ? whole : whole.narrow(1, 0, cols);
 }
 // x [rows, cols] -> 8-bit numbers, scales [column blocks, rows]
 py::tuple fp8_quantize(const Tensor& x, int dt) {

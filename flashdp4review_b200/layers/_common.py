@@ -55,14 +55,14 @@ def dropout_spec(p, stream_id, x):
 
     The seed is drawn from torch's CPU generator, which torch.utils.checkpoint restores before it runs a pass again: a count
     of the layer's own would give the recomputed pass another mask than the one whose output the rest of the network has
-    seen.  A data-parallel rank's groups of elements are numbered from its rank times 2^40.  With the device counter on
-    (a step captured in a graph) the step is its value now, copied on the stream, since it may have moved on by the time the
-    backward runs."""
+    seen.  A data-parallel rank's elements are numbered behind those of the ranks before it, as many as its own: equal
+    shards draw what the whole batch would.  With the device counter on (a step captured in a graph) the step is its value
+    now, copied on the stream, since it may have moved on by the time the backward runs."""
     counter = runtime.device_noise_counter(x.device) if x.is_cuda else None
     if counter is None and x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a captured dropout would draw the same mask on every replay: call use_device_noise_step() first")
     return ops.DropoutSpec(p=p, seed=int(torch.randint(-2 ** 63, 2 ** 63 - 1, (), device="cpu")) & (2 ** 64 - 1), stream_id=stream_id,
-                           offset=runtime.data_parallel()[0] << 40,
+                           offset=runtime.data_parallel()[0] * ((x.numel() + 7) // 8),
                            step_device=None if counter is None else counter.clone())
 
 
