@@ -28,8 +28,8 @@ __device__ __forceinline__ void dropout_some(const T* x, const T* residual, T* y
 // threads have 64 to 128 bytes each in flight.  x, residual and y may be one buffer: an element is read before it is
 // written, by the same thread.
 //
-// 134 M elements bf16: 94 us, 82 at the speed of a copy; 127 instructions a group of eight, 64 of them on the integer pipe, which
-// is 64% busy.  (Two groups a thread loaded into registers, 76 of them: 119.)
+// 134 M elements bf16: 94 to 98 us, 82 at the speed of a copy; 124 instructions a group of eight, 64 of them on the integer
+// pipe, which is 65% busy.  (Two groups a thread loaded into registers, 76 of them: 119.)
 template <typename T, bool VEC, bool RES>
 __global__ void __launch_bounds__(DROP_THREADS, DROP_PER_SM) dropout_kernel(const T* x, const T* residual, T* y, uint64_t n, const __grid_constant__ DropKey key) {
   constexpr int PARTS = sizeof(T) / 2, COPIES = PARTS * (RES ? 2 : 1), D = COPIES == 1 ? 4 : COPIES == 2 ? 3 : 2;

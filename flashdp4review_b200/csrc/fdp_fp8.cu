@@ -241,6 +241,9 @@ __global__ void __launch_bounds__(256) fp8_weight_kernel(const T* __restrict__ w
 // (Before: kind::f8f6f4 and the scales in the epilogue, where a K block's accumulator was added to fp32 registers times both
 // scales.  A hand-off is a commit, a wait, the accumulator's loads and an arrival across the pair, with two accumulators in
 // turn about 900 cycles for every 512 cycles of matrix instructions: 8192 rows 4096 -> 11008 386 us.)
+// (Tried: tiles of 256 x 192 with two accumulators, so that a pair's store runs beside the next tile's products.  What long thin
+// products wait for is their operands from L2, of which smaller tiles read more: with the quantisation of 16384 rows
+// 1024 -> 4096 78 us against 70, 8192 rows 4096 -> 11008 300 against 284, 8192 rows 2048 -> 2048 55 against 60.)
 //
 // The tensor cores add into their fp32 accumulators by truncation, one unit in the last place a step and all of one sign:
 // with 16-bit outputs that is nothing (344 steps at 11008 columns, 2^-16), with fp32 outputs an accumulator is handed over

@@ -10,8 +10,10 @@
 // Each direction reads its inputs twice, reductions first, then the result; the second pass runs from the back, so that what
 // the first one read last is still in L2.  A row is C contiguous numbers; a thread keeps one column (16 bytes) of channels
 // and walks rows, so that channel sums and parameters stay in registers.  All sums run in a fixed order.  What bounds it is
-// instruction issue as much as memory: at the memory's speed a 16-bit element leaves 22 issue slots a read and write, the
-// passes with an activation take 9 to 22, and what a block does beside its rows is worth six rows a thread more.
+// instruction issue as much as memory: at the memory's speed a 16-bit element leaves 22 issue slots for a read and a write or two
+// reads; the statistics take 10, the other passes 14 to 18 with silu and 25 to 33 with gelu and dropout, a third of that
+// what a block does beside its rows.  16 x 4096 x 320 bf16 with silu: 83 us both ways, from cold 13, 23, 26 and 27 a pass (the
+// reads and writes of both ways once: 32); 8 x 16384 x 256 fp32, whose tensors do not stay in L2: 193 us of 164.
 // (Tried: one kernel a direction whose blocks draw reductions and results from a counter, so that nothing drains between the
 // passes.  A block that drew a result waited for reductions still running beside it: 16 x 4096 x 320 bf16 144 us for both
 // directions against 117 then with a kernel a pass.  Tried: sets of samples whose second pass finds all of them in L2:
@@ -1043,9 +1045,9 @@ int bwd_drop(const GnArgs& a, const GnPlan& pl, bool need_dw, int* nparts, cudaS
 // How the work is cut up.  Must not depend on the device in use, nor on pointers: the workspace query has to agree.
 //
 // Small tensors, where launches are what counts: clusters.  A sample's groups go to `slabs` clusters, its rows to the `chunks`
-// blocks of each, and both passes are one kernel (4 x 64 x 128 fp32, forward and backward 10.6 + 15.7 us, with two kernels 13.4 + 17.8).
-// Others: a kernel a pass over whole rows, which keeps the SMs fuller (16 x 4096 x 320 bf16: 91 us, in clusters of 16 blocks 113
-// to 142), in the number of chunks that takes the fewest (rows a thread + fixed cost of a block) a wave of blocks.
+// blocks of each, and both passes are one kernel (4 x 64 x 128 fp32, forward and backward 10.6 + 15.7 us with the host, with two kernels 13.4 + 17.8; on the device alone 15.2 both).
+// Others: a kernel a pass over whole rows, which keeps the SMs fuller (16 x 4096 x 320 bf16: 91 us then, in clusters of 16 blocks
+// 113 to 142), in the number of chunks that takes the fewest (rows a thread + fixed cost of a block) a wave of blocks.
 GnPlan gn_plan(int B, int T, int C, int G, int element, int tensors, bool drop) {
   constexpr int FIXED_ROWS = 6, SEGMENT = 64;          // rows a thread that a block's fixed cost is worth; bytes of a slab's row
   constexpr long long PIECE = 96 << 10, SMALL = 2 << 20;
