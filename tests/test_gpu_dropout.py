@@ -108,3 +108,28 @@ def test_backward_is_the_same_mask(ops):
     s = ops.DropoutSpec(p=0.4, seed=8, stream_id=1, step=1)
     dx = ops.dropout_backward(g, s)
     assert torch.equal(dx != 0, ops.dropout(torch.ones_like(g), s) != 0)
+
+
+def test_more_than_2_32_elements(ops):
+    """In place; what stands for any stretch is what a tensor of its length draws with the stretch's first group as offset."""
+    n = 2 ** 32 + 24
+    base = dict(p=0.3, seed=11, stream_id=4, step=9)
+    x = torch.ones(n, dtype=torch.float16, device=dev())
+    assert ops.dropout(x, ops.DropoutSpec(**base), out=x) is not None
+    ones = torch.ones(4104, dtype=torch.float16, device=dev())
+    for start in (0, 2 ** 31 - 2048, 2 ** 32 - 4096, n - 4104):
+        assert torch.equal(x[start:start + 4104], ops.dropout(ones, ops.DropoutSpec(**base, offset=start // 8)))
+
+
+def test_two_streams_at_once(ops):
+    x = torch.randn(3, 1 << 20, device=dev())
+    specs = [ops.DropoutSpec(p=0.25, seed=s) for s in range(3)]
+    want = [ops.dropout(x[i], specs[i]) for i in range(3)]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for i, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            got.append(ops.dropout(x[i], specs[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

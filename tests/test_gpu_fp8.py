@@ -134,3 +134,22 @@ def test_repeated_calls_give_the_same_bits(ops):
         a = ops.fp8_linear_forward(x, w8)
         for _ in range(3):
             assert torch.equal(a, ops.fp8_linear_forward(x, w8))
+
+
+@pytest.mark.parametrize("N,K", [(64, 2056), (2056, 128), (2057, 128)])
+def test_more_than_2_31_elements(ops, N, K):
+    """Rows at the end of an operand or a result with more than 2^31 numbers are what they are by themselves (in tiles and orders of
+    accumulation that may be others: 48 + 8 a K block roundings at most on either side)."""
+    M, last = 2 ** 20 + 136, 300
+    gen = torch.Generator().manual_seed(6)
+    x = torch.randn(4096, K, generator=gen).to(torch.bfloat16).to(dev()).repeat(257, 1)[:M]
+    x[-last:] = torch.randn(last, K, generator=gen).to(torch.bfloat16).to(dev())
+    w = torch.randn(N, K, generator=gen).to(torch.bfloat16).to(dev())
+    w8 = ops.fp8_quantize_weight(w)
+    assert x.numel() > 2 ** 31 or M * N > 2 ** 31
+    y = ops.fp8_linear_forward(x, w8)
+    few = ops.fp8_linear_forward(x[-last:], w8, out_dtype=torch.float32)
+    mag = ops.fp8_linear_forward(x[-last:].abs(), ops.fp8_quantize_weight(w.abs()), out_dtype=torch.float32)
+    tol = torch.finfo(torch.bfloat16).eps / 2 * few.abs() + 2 * (48 + 8 * -(-K // 128)) * 2.0 ** -24 * mag * 1.01
+    assert ((y[-last:].float() - few).abs() <= tol).all()
+    assert torch.equal(y[4096 * 254:4096 * 255], y[:4096])      # (of the 256th stretch 164 rows are among the last)

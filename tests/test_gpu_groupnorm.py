@@ -197,3 +197,60 @@ def test_noise_divisor_and_repeatability(ops):
     for k, pid in ((1, 5), (2, 6)):
         z = torch.from_numpy(O.gaussian_noise(64, 0.5, 77, pid, 2))
         assert ((r1[k] - r0[k]).double().cpu() - z).abs().max() < 3e-6
+
+
+def test_many_chunks_and_many_samples(ops):
+    """Statistics put together by a launch of their own (more than 64 chunks a sample), and more samples than the clipped sum keeps
+    factors of in shared memory."""
+    check(ops, *case(1, 9001, 96, torch.bfloat16, seed=3), 6, "silu")
+    check(ops, *case(1, 9001, 96, torch.float32, seed=4), 6, None)
+    B, T, C, G = 9000, 2, 8, 2
+    x, dy, w, b = case(B, T, C, torch.float32, seed=5)
+    y, mean, rstd, xhat, z = P.group_norm(x, w, b, G, 1e-5, None, None, 0.0)
+    _, st = ops.group_norm_forward(x.to(dev()), w.to(dev()), b.to(dev()), G)
+    res = ops.dp_group_norm_backward(dy.to(dev()), x.to(dev()), w.to(dev()), b.to(dev()), st["mean"], st["rstd"], G, 0.1, 1.0, return_norms=True)
+    want = P.group_norm_backward(dy, w, rstd, xhat, z, G, None, None, 0.0)
+    xerr = FP32 * ((x.double().abs() + mean.abs().repeat_interleave(C // G, 1)[:, None]) * rstd.repeat_interleave(C // G, 1)[:, None] + 2)
+    for got, norms, name, more in ((res[1], res[3], "dgamma", (dy.double().abs() * xerr).sum(1)), (res[2], res[4], "dbeta", 0.0)):
+        per, mag = want[name]
+        mean_, n_ = P.clipped_mean(per, 0.1, 1.0)
+        err = FP32 * mag + more
+        nerr = err.square().sum(1).sqrt() + FP32 * n_
+        assert ((norms.double().cpu() - n_).abs() <= nerr + 1e-30).all()
+        f = torch.from_numpy(O.clip_factor(n_.numpy(), 0.1, 1.0))
+        # the sum over the samples is a chain of at most B additions, each off by 2^-24 of the magnitudes so far
+        tol = (err * f[:, None] + per.abs() * (f * (nerr / n_.clamp(min=1e-30) + FP32 + B * 2.0 ** -24))[:, None]).sum(0) / B
+        close(got, mean_, torch.zeros_like(mean_), torch.float32, tol)
+
+
+def test_more_than_2_31_elements(ops):
+    """Samples of 512 equal stretches: their statistics and the sums of the backward are a stretch's (times 512), and every stretch
+    of a result has the same bits.  A thread's chain has fewer than 4096 rows (2^21 in at least 222 chunks and three row classes),
+    so sums are off by at most 2^-12 of their magnitudes, and the variance, which two of them make, by 2^-11."""
+    B, T, C, G, N = 2, 4096, 520, 8, 512
+    x, dy, w, b = case(B, T, C, torch.bfloat16, seed=6)
+    big_x, big_dy = x.to(dev()).repeat(1, N, 1), dy.to(dev()).repeat(1, N, 1)
+    assert big_x.numel() > 2 ** 31
+    y, st = ops.group_norm_forward(big_x, w.to(dev()), b.to(dev()), G, activation="silu")
+    got = y.view(B, N, T, C)
+    assert all(torch.equal(got[:, i], got[:, 0]) for i in range(1, N))
+    want, mean, rstd, xhat, z = P.group_norm(x, w, b, G, 1e-5, "silu", None, 0.0)
+    by = lambda a: a.repeat_interleave(C // G, 1)[:, None]
+    lost = 2.0 ** -11
+    zerr = lost * (((x.double().abs() + by(mean.abs())) * by(rstd) + 2) * w.double().abs() + b.double().abs())
+    close(got[:, 0], want, 1.13 * zerr / FP32, torch.bfloat16)
+    del y, got
+    res = ops.dp_group_norm_backward(big_dy, big_x, w.to(dev()), b.to(dev()), st["mean"], st["rstd"], G, 1e30, 1.0, activation="silu")
+    got = res[0].view(B, N, T, C)
+    assert all(torch.equal(got[:, i], got[:, 0]) for i in range(1, N))
+    back = P.group_norm_backward(dy, w, rstd, xhat, z, G, "silu", None, 0.0)
+    gerr = 1.13 * zerr * dy.double().abs() + lost * back["gz"].abs()          # of gz: |act''| <= 1.13
+    grp = lambda a: by(a.reshape(B, T, G, C // G).sum((1, 3)) / (T * C // G))
+    gmul = w.double().abs()
+    xerr = lost * ((x.double().abs() + by(mean.abs())) * by(rstd) + 2)
+    u = back["gz"].abs() * gmul
+    extra = by(rstd) * (gerr * gmul + grp(gerr * gmul) + xhat.abs() * grp(gerr * gmul * xhat.abs() + u * xerr) + xerr * grp(u * xhat.abs()))
+    close(got[:, 0], back["dx"][0], back["dx"][1] * lost / FP32, torch.bfloat16, extra)
+    for g, name, more in ((res[1], "dgamma", (gerr * xhat.abs() + back["gz"].abs() * xerr).sum(1)), (res[2], "dbeta", gerr.sum(1))):
+        per, mag = back[name]
+        close(g, N * per.mean(0), torch.zeros(C), torch.float32, N * (lost * mag + more).mean(0))
