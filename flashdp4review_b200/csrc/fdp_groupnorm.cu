@@ -390,6 +390,10 @@ __device__ __forceinline__ void for_groups(int G, int lanes, Body body) {
   }
 }
 
+// Where the sums of channel c lie in shared memory, two floats each: a thread writes those of V adjacent channels, and with these in
+// order the lanes of a warp would be 8 V bytes apart, V (of up to eight) on the same banks.
+template <int V> __device__ __forceinline__ int spread(int c) { return c ^ ((c >> 4) & (V - 1)); }
+
 // ---- forward, first pass: mean and sum of squared deviations of every (sample, chunk, group) ------------
 // A thread takes its sums about the first number that it sees of a channel: the squares then lose nothing to a mean that is
 // large against the spread, and a first number far off the others is itself part of the spread (n deviations about it lose
@@ -427,7 +431,7 @@ __device__ __forceinline__ void gn_stats(const Shape& h, const Share& sh, const 
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float m = f1[e] * inv;
-      gn_ent[static_cast<size_t>(pl.row) * C + col * V + e] = make_float2(m - fp[e], fmaxf(f2[e] - f1[e] * m, 0.f));
+      gn_ent[pl.row * C + spread<V>(col * V + e)] = make_float2(m - fp[e], fmaxf(f2[e] - f1[e] * m, 0.f));
     }
   }
   __syncthreads();
@@ -435,29 +439,30 @@ __device__ __forceinline__ void gn_stats(const Shape& h, const Share& sh, const 
   const int classes = min(pl.rg, span_rows), base_rows = quotient(span_rows, pl.rg, h.by_rg), longer = span_rows - base_rows * pl.rg;
   const float inv = 1.f / max(1, span_rows);
   for (int c = threadIdx.x; c < C; c += GN_THREADS) {
-    const float2 first = gn_ent[c];
+    float2* e = gn_ent + spread<V>(c);
+    const float2 first = e[0];
     float sum = 0.f, m2 = first.y;
-    for (int k = 1; k < classes; ++k) sum = fmaf(static_cast<float>(base_rows + (k < longer)), gn_ent[static_cast<size_t>(k) * C + c].x - first.x, sum);
+    for (int k = 1; k < classes; ++k) sum = fmaf(static_cast<float>(base_rows + (k < longer)), e[k * C].x - first.x, sum);
     const float m = sum * inv;               // the channel's mean, less the first class's
     m2 = fmaf(static_cast<float>(base_rows + (0 < longer)) * m, m, m2);
     for (int k = 1; k < classes; ++k) {
-      const float2 v = gn_ent[static_cast<size_t>(k) * C + c];
+      const float2 v = e[k * C];
       const float d = v.x - first.x - m;
       m2 += fmaf(static_cast<float>(base_rows + (k < longer)) * d, d, v.y);
     }
-    gn_ent[c] = make_float2(first.x + m, m2);
+    e[0] = make_float2(first.x + m, m2);
   }
   __syncthreads();
   const int cg = h.cg, lanes = h.lanes_channels;
   for_groups(G, lanes, [&](int g, int k, bool valid) {
-    const float2* e = gn_ent + g * cg;
-    const float ref = e[0].x;
+    const int c0 = g * cg;
+    const float ref = gn_ent[spread<V>(c0)].x;
     float sum = 0.f;
-    for (int c = k; c < cg; c += lanes) sum += e[c].x - ref;
+    for (int c = k; c < cg; c += lanes) sum += gn_ent[spread<V>(c0 + c)].x - ref;
     const float mean = fmaf(lanes_sum(sum, lanes), h.inv_cg, ref);
     float m2 = 0.f;
     for (int c = k; c < cg; c += lanes) {
-      const float2 v = e[c];
+      const float2 v = gn_ent[spread<V>(c0 + c)];
       const float d = v.x - mean;
       m2 += fmaf(span_rows * d, d, v.y);
     }
@@ -497,7 +502,31 @@ __device__ __forceinline__ Nums<V> take_v(const float* s, int col) {
 
 // (mean, squared deviations) of a sample's group from its chunks', by `lanes` threads.  (From L2: in a cluster the others' are new.)
 __device__ __forceinline__ float2 gn_moments(const Shape& h, const float2* p, int chunks, int rows_per_chunk, int lanes, int k) {
+  constexpr int KEEP = 8;
   const float ref = __ldcg(p).x;
+  if (chunks <= KEEP * lanes) {                // (one way to L2 instead of two)
+    float2 v[KEEP];
+    float rows[KEEP], sum = 0.f, m2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+      const int i = k + j * lanes;
+      rows[j] = 0.f;
+      v[j] = make_float2(ref, 0.f);
+      if (i < chunks) {
+        rows[j] = static_cast<float>(max(0, min(rows_per_chunk, h.T - i * rows_per_chunk)));
+        if (rows[j] > 0.f) v[j] = __ldcg(p + static_cast<size_t>(i) * h.allG);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) sum = fmaf(rows[j], v[j].x - ref, sum);
+    const float off = lanes_sum(sum, lanes) * h.inv_T;
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+      const float d = v[j].x - ref - off;
+      m2 += fmaf(rows[j] * h.cg * d, d, v[j].y);
+    }
+    return make_float2(ref + off, lanes_sum(m2, lanes));
+  }
   float sum = 0.f;
 #pragma unroll 4
   for (int i = k; i < chunks; i += lanes) {
@@ -556,7 +585,11 @@ __device__ __forceinline__ void gn_apply(const Shape& h, const Share& sh, const 
   float2* stat = reinterpret_cast<float2*>(c_b + cp);
   Stream in;
   in.src[0] = x + share_start(h, sh);
-  int n = gn_begin(in, gn_raw, h, sh, pl, V, pl.col);                // (the rows need not wait for their statistics)
+  int n = gn_begin(in, gn_raw, h, sh, pl, V, pl.col);                // (rows and parameters need not wait for the statistics)
+  for (int c = threadIdx.x; c < C; c += GN_THREADS) {
+    c_a[c] = q.gamma != nullptr ? load_as(q.gamma, q.pdt, sh.c0 + c) : 1.f;
+    c_b[c] = q.beta != nullptr ? load_as(q.beta, q.pdt, sh.c0 + c) : 0.f;
+  }
   wait();
   const int lanes = merge_chunks == h.chunks ? h.lanes_chunks : 1, rows = merge_chunks == h.chunks ? h.rows_per_chunk : h.T;
   for_groups(G, lanes, [&](int g, int k, bool valid) {
@@ -574,8 +607,7 @@ __device__ __forceinline__ void gn_apply(const Shape& h, const Share& sh, const 
   for (int c = threadIdx.x; c < C; c += GN_THREADS) {
     const float2 st = stat[small_quotient(c, h.inv_cg)];
     c_mu[c] = -st.x;
-    c_a[c] = q.gamma != nullptr ? st.y * load_as(q.gamma, q.pdt, sh.c0 + c) : st.y;
-    c_b[c] = q.beta != nullptr ? load_as(q.beta, q.pdt, sh.c0 + c) : 0.f;
+    c_a[c] *= st.y;
   }
   __syncthreads();
   if (!pl.on) return;
@@ -627,6 +659,7 @@ __global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_fwd_cluster_ke
   const Share sh = cluster_share(h);
   const Place pl = place_of(h);
   gn_stats<T, V>(h, sh, pl, gn_raw, x, part);
+  __syncthreads();
   gn_apply<T, V, DROP>(h, sh, pl, gn_raw, x, part, h.chunks, y, q, key, [] { cluster_meet(); });
 }
 
@@ -693,7 +726,7 @@ __device__ __forceinline__ void gn_bwd_sums(const Shape& h, const Share& sh, con
     n_get<V>(t2, s2);
     if (apart) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) reinterpret_cast<float2*>(wide)[col * V + e] = make_float2(s1[e], s2[e]);
+      for (int e = 0; e < V; ++e) reinterpret_cast<float2*>(wide)[spread<V>(col * V + e)] = make_float2(s1[e], s2[e]);
     }
   }
   __syncthreads();
@@ -702,27 +735,27 @@ __device__ __forceinline__ void gn_bwd_sums(const Shape& h, const Share& sh, con
   } else {
     if (pl.on) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) ent[static_cast<size_t>(pl.row) * C + pl.col * V + e] = make_float2(s1[e], s2[e]);
+      for (int e = 0; e < V; ++e) ent[pl.row * C + spread<V>(pl.col * V + e)] = make_float2(s1[e], s2[e]);
     }
     __syncthreads();
   }
   const size_t at = (static_cast<size_t>(sh.b) * h.chunks + sh.chunk) * h.allC + sh.c0, second = static_cast<size_t>(h.B) * h.chunks * h.allC;
   for (int c = threadIdx.x; c < C; c += GN_THREADS) {
-    float2 t = ent[c];
-    for (int k = 1; k < pl.rg; ++k) { const float2 v = ent[static_cast<size_t>(k) * C + c]; t.x += v.x; t.y += v.y; }
+    float2* e = ent + spread<V>(c);
+    float2 t = e[0];
+    for (int k = 1; k < pl.rg; ++k) { const float2 v = e[k * C]; t.x += v.x; t.y += v.y; }
     t.y *= __ldg(q.rstd + static_cast<size_t>(sh.b) * h.allG + sh.g0 + small_quotient(c, h.inv_cg));
     part[at + c] = t.y;
     part[second + at + c] = t.x;
     const float ga = q.gamma != nullptr ? load_as(q.gamma, q.pdt, sh.c0 + c) : 1.f;
-    ent[c] = make_float2(ga * t.x, ga * t.y);
+    e[0] = make_float2(ga * t.x, ga * t.y);
   }
   if (gpart == nullptr) return;
   __syncthreads();
   const int lanes = h.lanes_channels;
   for_groups(G, lanes, [&](int g, int k, bool valid) {
-    const float2* e = ent + g * cg;
     float u = 0.f, v = 0.f;
-    for (int c = k; c < cg; c += lanes) { u += e[c].x; v += e[c].y; }
+    for (int c = k; c < cg; c += lanes) { const float2 e = ent[spread<V>(g * cg + c)]; u += e.x; v += e.y; }
     u = lanes_sum(u, lanes);
     v = lanes_sum(v, lanes);
     if (valid && k == 0) gpart[(static_cast<size_t>(sh.b) * h.chunks + sh.chunk) * h.allG + sh.g0 + g] = make_float2(u, v);
@@ -774,8 +807,8 @@ __device__ __forceinline__ void gn_bwd_dx(const Shape& h, const Share& sh, const
   in.src[0] = dy + share_start(h, sh);
   in.src[1] = x + share_start(h, sh);
   int n = gn_begin(in, gn_raw, h, sh, pl, V, pl.col);
-  wait();
   bwd_constants(c_mu, c_a, c_b, q.gamma, q.beta, q.mean, q.rstd, q.pdt, h, sh);
+  wait();
   const float inv_n = h.inv_n;
   const int lanes = merge_chunks == h.chunks ? h.lanes_chunks : h.lanes_channels;
   for_groups(G, lanes, [&](int g, int k, bool valid) {
