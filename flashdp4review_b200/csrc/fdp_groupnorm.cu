@@ -12,8 +12,9 @@
 // and walks rows, so that channel sums and parameters stay in registers.  All sums run in a fixed order.  What bounds it is
 // instruction issue as much as memory: at the memory's speed a 16-bit element leaves 22 issue slots for a read and a write or two
 // reads; the statistics take 10, the other passes 14 to 18 with silu and 25 to 33 with gelu and dropout, a third of that
-// what a block does beside its rows.  16 x 4096 x 320 bf16 with silu: 83 us both ways, from cold 13, 23, 26 and 27 a pass (the
-// reads and writes of both ways once: 32); 8 x 16384 x 256 fp32, whose tensors do not stay in L2: 193 us of 164.
+// what a block does beside its rows.  16 x 4096 x 320 bf16 with silu: 80 us both ways (the reads and writes of both
+// ways once: 32); with 16 x 324 x 320 a pass takes 7 to 13 us from cold, so its start and end are much of it.  8 x 16384 x 256
+// fp32, whose tensors do not stay in L2: 191 us of 164.
 // (Tried: one kernel a direction whose blocks draw reductions and results from a counter, so that nothing drains between the
 // passes.  A block that drew a result waited for reductions still running beside it: 16 x 4096 x 320 bf16 144 us for both
 // directions against 117 then with a kernel a pass.  Tried: sets of samples whose second pass finds all of them in L2:
@@ -29,7 +30,7 @@ namespace {
 constexpr int GN_THREADS = 256, GN_WARPS = GN_THREADS / 32;
 // blocks an SM holds, by their registers: with the generator's words and keys beside the numbers only two
 constexpr int gn_per_sm(bool drop) { return drop ? 2 : 3; }
-// rows a turn of the loops: with the mask's draw two at once only lengthen the code (16 x 1024 x 1024 bf16: 107 us against 104)
+// rows a turn of the loops: with the mask's draw two at once only lengthen the code (16 x 1024 x 1024 bf16: 107 us against 104 then)
 __host__ __device__ constexpr int gn_unroll(bool drop) { return drop ? 1 : 2; }
 
 // ---- V numbers of a thread --------------------------------------------------------------------------
