@@ -12,7 +12,7 @@
 // and walks rows, so that channel sums and parameters stay in registers.  All sums run in a fixed order.  What bounds it is
 // instruction issue as much as memory: at the memory's speed a 16-bit element leaves 22 issue slots for a read and a write or two
 // reads; the statistics take 10, the other passes 14 to 18 with silu and 25 to 33 with gelu and dropout, a third of that
-// what a block does beside its rows.  16 x 4096 x 320 bf16 with silu: 80 us both ways (the reads and writes of both
+// what a block does beside its rows.  16 x 4096 x 320 bf16 with silu: 77 us both ways (the reads and writes of both
 // ways once: 32); with 16 x 324 x 320 a pass takes 7 to 13 us from cold, so its start and end are much of it.  8 x 16384 x 256
 // fp32, whose tensors do not stay in L2: 191 us of 164.
 // (Tried: one kernel a direction whose blocks draw reductions and results from a counter, so that nothing drains between the
@@ -841,19 +841,21 @@ __device__ __forceinline__ void gn_bwd_dx(const Shape& h, const Share& sh, const
   }
 }
 
-// The launch has blocks in front that form the per-sample gradients, which need the first pass only: no launch of their own.
+// The launch has blocks behind those of dx that form the per-sample gradients, which need the first pass only: no launch of their
+// own.  (In front they kept the others from starting: 16 x 4096 x 320 bf16 80 us both ways, now 77.)
 struct GnPsgrad { int pieces; const float* part; float *out, *sumsq; };
 template <typename T, int V, bool DROP>
 __global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_bwd_dx_kernel(const Shape h, const T* dy, const T* x, const GnBwd q, const float2* gpart,
                                                                              int merge_chunks, T* dx, const GnPsgrad ps, const DropKey key) {
   extern __shared__ __align__(16) uint8_t gn_raw[];
   pdl_trigger();
-  if (static_cast<int>(blockIdx.x) < ps.pieces) {
+  const int blocks = static_cast<int>(gridDim.x) - ps.pieces;
+  if (static_cast<int>(blockIdx.x) >= blocks) {
     pdl_wait();
-    gn_psgrad(blockIdx.x, reinterpret_cast<float*>(gn_raw), ps.part, ps.out, ps.sumsq, h.chunks, h.C);
+    gn_psgrad(blockIdx.x - blocks, reinterpret_cast<float*>(gn_raw), ps.part, ps.out, ps.sumsq, h.chunks, h.C);
     return;
   }
-  gn_bwd_dx<T, V, DROP>(h, share_of(h, gridDim.x - 1 - blockIdx.x), place_of(h), gn_raw, dy, x, q, gpart, merge_chunks, dx, key,
+  gn_bwd_dx<T, V, DROP>(h, share_of(h, blocks - 1 - blockIdx.x), place_of(h), gn_raw, dy, x, q, gpart, merge_chunks, dx, key,
                               [] { pdl_wait(); });
 }
 // In a cluster every block also forms its part of the sample's gradients: one of h.chunks stretches of the channels.
