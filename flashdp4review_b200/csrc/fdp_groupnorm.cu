@@ -896,9 +896,9 @@ __global__ void __launch_bounds__(GN_THREADS, gn_per_sm(DROP)) gn_bwd_cluster_ke
   else gradients();
 }
 
-// clip factors from the sums of squares, clipped sum over the samples, mean, noise: 32 columns of one tensor a block, eight
-// threads a column
-__global__ void __launch_bounds__(GN_THREADS) gn_clip_kernel(const float* psgrad, const float* sumsq, int nparts, float Cc, float clamp, float* norms0,
+// clip factors from the sums of squares (`lanes` threads a sample), clipped sum over the samples, mean, noise: 32 columns of one
+// tensor a block, eight threads a column, whose first numbers are on their way while the factors are formed
+__global__ void __launch_bounds__(GN_THREADS) gn_clip_kernel(const float* psgrad, const float* sumsq, int nparts, int lanes, float Cc, float clamp, float* norms0,
                                                              float* norms1, void* out0, void* out1, int B, int C, int out_dt, float inv_div, NoiseKey nk0,
                                                              NoiseKey nk1) {
   extern __shared__ __align__(16) uint8_t gn_raw[];
@@ -906,31 +906,44 @@ __global__ void __launch_bounds__(GN_THREADS) gn_clip_kernel(const float* psgrad
   __shared__ float red[GN_THREADS];
   const int tensor = blockIdx.y, l = threadIdx.x & 31, k0 = threadIdx.x >> 5, c = blockIdx.x * 32 + l;
   pdl_wait();
-  for (int b = threadIdx.x; b < B; b += GN_THREADS) {
-    const float* p = sumsq + (static_cast<size_t>(tensor) * B + b) * nparts;
-    float sq = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < nparts; ++i) sq += p[i];
-    const float n = norm_of_sumsq(sq);
-    fac[b] = clip_factor(n, Cc, clamp);
-    float* no = tensor == 0 ? norms0 : norms1;
-    if (blockIdx.x == 0 && no != nullptr) no[b] = n;
+  constexpr int AHEAD = 8;
+  const float* p = psgrad + static_cast<size_t>(tensor) * B * C + c;
+  float v[AHEAD];
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) {
+    const int b = k0 + j * GN_WARPS;
+    v[j] = c < C && b < B ? p[static_cast<size_t>(b) * C] : 0.f;
   }
+  for_groups(B, lanes, [&](int b, int k, bool valid) {
+    const float* part = sumsq + (static_cast<size_t>(tensor) * B + b) * nparts;
+    float sq = 0.f;
+#pragma unroll 4
+    for (int i = k; i < nparts; i += lanes) sq += part[i];
+    sq = lanes_sum(sq, lanes);
+    if (valid && k == 0) {
+      const float n = norm_of_sumsq(sq);
+      fac[b] = clip_factor(n, Cc, clamp);
+      float* no = tensor == 0 ? norms0 : norms1;
+      if (blockIdx.x == 0 && no != nullptr) no[b] = n;
+    }
+  });
   __syncthreads();
   float acc = 0.f;
-  const float* p = psgrad + static_cast<size_t>(tensor) * B * C + c;
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j)
+    if (k0 + j * GN_WARPS < B) acc = fmaf(fac[k0 + j * GN_WARPS], v[j], acc);
   if (c < C)
 #pragma unroll 8
-    for (int b = k0; b < B; b += GN_WARPS) acc = fmaf(fac[b], p[static_cast<size_t>(b) * C], acc);
+    for (int b = k0 + AHEAD * GN_WARPS; b < B; b += GN_WARPS) acc = fmaf(fac[b], p[static_cast<size_t>(b) * C], acc);
   red[threadIdx.x] = acc;
   __syncthreads();
   if (k0 == 0 && c < C) {
 #pragma unroll
     for (int k = 1; k < GN_WARPS; ++k) acc += red[k * 32 + l];
-    float v = acc * inv_div;
+    float mean = acc * inv_div;
     const NoiseKey& nk = tensor == 0 ? nk0 : nk1;
-    if (nk.std != 0.f) v += noise_at(nk, c);
-    store_as(tensor == 0 ? out0 : out1, out_dt, c, v);
+    if (nk.std != 0.f) mean += noise_at(nk, c);
+    store_as(tensor == 0 ? out0 : out1, out_dt, c, mean);
   }
 }
 
@@ -1149,7 +1162,7 @@ int gn_bwd(const GnArgs& a, int dt, const fdp_dp_params* p, void* dgamma, void* 
   const float inv_div = 1.0f / static_cast<float>(div);
   const NoiseKey nk0 = make_noise_key(p, p->param_id), nk1 = make_noise_key(p, p->param_id2);
   if (a.B <= 8192) {
-    launch_dependent(gn_clip_kernel, dim3(ceil_div(a.C, 32), 2), dim3(GN_THREADS), sizeof(float) * a.B, s, a.psgrad, a.sumsq, nparts, p->C,
+    launch_dependent(gn_clip_kernel, dim3(ceil_div(a.C, 32), 2), dim3(GN_THREADS), sizeof(float) * a.B, s, a.psgrad, a.sumsq, nparts, group_lanes(a.B, nparts), p->C,
                      p->clamp_value, norms_gamma, norms_beta, dgamma, dbeta, a.B, a.C, a.pdt, inv_div, nk0, nk1);
     note_launch();
   } else {
