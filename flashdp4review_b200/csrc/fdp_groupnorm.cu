@@ -1094,7 +1094,10 @@ int bwd_drop(const GnArgs& a, const GnPlan& pl, bool need_dw, int* nparts, cudaS
 // How the work is cut up.  Must not depend on the device in use, nor on pointers: the workspace query has to agree.
 //
 // Small tensors, where launches are what counts: clusters.  A sample's groups go to `slabs` clusters, its rows to the `chunks`
-// blocks of each, and both passes are one kernel (4 x 64 x 128 fp32, forward and backward 10.6 + 15.7 us with the host, with two kernels 13.4 + 17.8; on the device alone 15.2 both).
+// blocks of each, and both passes are one kernel.  On the device a kernel a pass is as fast or faster (16 x 64 x 256 bf16, forward
+// and backward 5.8 + 8.5 us against 6.9 + 9.8; 2 x 1600 x 256 13.0 + 14.3 against 8.8 + 14.3), but up to 2 MB a call takes the host
+// longer than either, and a launch more is 2 to 3 us of it.  (Rows of a slab are at least 64 bytes, where they are no vectors 32:
+// 3 x 1369 x 90 fp16 backward 13.1 us with one slab, 11.8 with three.)
 // Others: a kernel a pass over whole rows, which keeps the SMs fuller (16 x 4096 x 320 bf16: 91 us then, in clusters of 16 blocks
 // 113 to 142), in the number of chunks that takes the fewest (rows a thread + fixed cost of a block) a wave of blocks.
 GnPlan gn_plan(int B, int T, int C, int G, int element, int tensors, bool drop) {
@@ -1112,7 +1115,7 @@ GnPlan gn_plan(int B, int T, int C, int G, int element, int tensors, bool drop) 
     for (int d = 1; d <= G; ++d) {
       if (G % d != 0) continue;
       const int cs = C / d;
-      if (d > 1 && cs * element < SEGMENT) break;
+      if (d > 1 && cs * element < (pl.vec == wide ? SEGMENT : SEGMENT / 2)) break;
       if (cs % pl.vec != 0) continue;
       const int most = ceil_div(T, 2 * rows_at_a_time(cs / pl.vec));            // chunks of at least two rows a thread
       int k = 1;
