@@ -1,4 +1,5 @@
 """Shared pieces of the DP layer backward passes."""
+import collections
 import weakref
 
 import torch
@@ -50,20 +51,79 @@ def dp_scalars(local_batch, noise_multiplier, param_id, step, param_id2=0):
                                    step_device=runtime.device_noise_counter() if std != 0.0 else None)
 
 
-def dropout_spec(p, stream_id, x):
+# The specs of passes that drew at a step of the device counter, by (device, seed, stream): a pass that
+# torch.utils.checkpoint runs again finds the step of the first one there.  A pass's graph keeps its spec; one that leaves no graph (the
+# first pass of a reentrant checkpoint, or a dropout of something that needs no gradient) is kept in `_graphless`.
+_drawn = {}
+_graphless = collections.deque()
+_GRAPHLESS_MOST = 1 << 14
+_forgotten = False                  # a spec that nothing had asked for again was dropped from there
+
+
+def _counter_of(x):
+    return runtime.device_noise_counter(x.device) if x.is_cuda else None
+
+
+def _remember(key, spec, graph):
+    global _forgotten
+
+    def gone(ref):
+        refs = [r for r in _drawn.get(key, ()) if r is not ref]
+        if refs:
+            _drawn[key] = refs
+        else:
+            _drawn.pop(key, None)
+
+    # (under a seed that is used again, what has been run again already is done with)
+    live = [r for r in _drawn.get(key, ()) if r() is not None and not r().run_again]
+    _drawn[key] = live + [weakref.ref(spec, gone)]
+    if not graph:
+        _graphless.append(spec)
+        if len(_graphless) > _GRAPHLESS_MOST:
+            _forgotten |= not _graphless.popleft().run_again
+
+
+def _first_pass(key):
+    """The spec that a pass which runs within a backward was first run with; None for one that was not."""
+    live = [s for s in (r() for r in _drawn.get(key, ())) if s is not None]
+    if len(live) > 1 and any(not torch.equal(s.step_device, live[0].step_device) for s in live[1:]):
+        raise RuntimeError("a dropout is run again for its gradient, but several passes drew from the same seed of torch's CPU generator "
+                           "at different steps: let go of the graphs of the earlier ones, or seed them differently")
+    if not live and _forgotten:
+        raise RuntimeError(f"a dropout is run again for its gradient, and more than {_GRAPHLESS_MOST} passes without a graph drew masks "
+                           "before it, so that its first pass is no longer known: checkpoint it with use_reentrant=False")
+    return live[0] if live else None
+
+
+def dropout_spec(p, stream_id, x, graph=True):
     """The mask of one forward pass of a dropout over as many elements as `x` has, for its backward to draw again.
+    `graph`: the pass leaves an autograd node, which keeps the spec.
 
     The seed is drawn from torch's CPU generator, which torch.utils.checkpoint restores before it runs a pass again: a count
     of the layer's own would give the recomputed pass another mask than the one whose output the rest of the network has
     seen.  A data-parallel rank's elements are numbered behind those of the ranks before it, as many as its own: equal
     shards draw what the whole batch would.  With the device counter on (a step captured in a graph) the step is its value
-    now, copied on the stream, since it may have moved on by the time the backward runs."""
-    counter = runtime.device_noise_counter(x.device) if x.is_cuda else None
+    now, copied on the stream, since it may have moved on by the time the backward runs; a pass that is run again within a backward, by
+    its seed, takes the copy of the first one."""
+    counter = _counter_of(x)
     if counter is None and x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a captured dropout would draw the same mask on every replay: call use_device_noise_step() first")
-    return ops.DropoutSpec(p=p, seed=int(torch.randint(-2 ** 63, 2 ** 63 - 1, (), device="cpu")) & (2 ** 64 - 1), stream_id=stream_id,
-                           offset=runtime.data_parallel()[0] * ((x.numel() + 7) // 8),
-                           step_device=None if counter is None else counter.clone())
+    spec = ops.DropoutSpec(p=p, seed=int(torch.randint(-2 ** 63, 2 ** 63 - 1, (), device="cpu")) & (2 ** 64 - 1), stream_id=stream_id,
+                           offset=runtime.data_parallel()[0] * ((x.numel() + 7) // 8))
+    if counter is not None:
+        key = (counter.device, spec.seed, stream_id)
+        first = _first_pass(key) if torch._C._current_graph_task_id() != -1 else None
+        if first is not None:
+            first.run_again = True
+            spec.step_device = first.step_device
+        else:
+            spec.step_device, spec.run_again = counter.clone(), False
+            _remember(key, spec, graph)
+    return spec
+
+
+def leaves_a_graph(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def direct_grad_target(param):

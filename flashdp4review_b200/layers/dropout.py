@@ -7,7 +7,7 @@ from torch.autograd.function import Function, once_differentiable
 
 from .. import runtime
 from ..core import ops
-from ._common import dropout_spec
+from ._common import dropout_spec, leaves_a_graph
 
 
 def _storage_order(x):
@@ -64,4 +64,5 @@ class DPDropout(nn.Dropout):
             return input if residual is None else input + residual
         if self.inplace and residual is not None:
             raise RuntimeError("dropout in place takes no residual")
-        return _DropoutFunc.apply(input, residual, dropout_spec(self.p, self._stream_id, input), self.inplace)
+        return _DropoutFunc.apply(input, residual, dropout_spec(self.p, self._stream_id, input, leaves_a_graph(input, residual)),
+                                  self.inplace)

@@ -9,7 +9,7 @@ from torch.autograd.function import Function, once_differentiable
 
 from ..core import ops
 from .utils import DPParameter as Parameter
-from ._common import DPLayerMixin, dp_scalars, dropout_spec
+from ._common import DPLayerMixin, dp_scalars, dropout_spec, leaves_a_graph
 
 
 class _DPGroupNormFunc(Function):
@@ -63,7 +63,7 @@ class DPGroupNorm(nn.GroupNorm, DPLayerMixin):
         x = input if self.channels_last else input.movedim(1, -1)
         spec = None
         if self.training and self.dropout > 0.0:
-            spec = dropout_spec(self.dropout, self._dp_param_ids[2], x)
+            spec = dropout_spec(self.dropout, self._dp_param_ids[2], x, leaves_a_graph(x, self.weight, self.bias))
         y = _DPGroupNormFunc.apply(x, self.weight, self.bias, self, spec)
         return y if self.channels_last else y.movedim(-1, 1)
 

@@ -1,0 +1,103 @@
+"""The layers of the operators around a stand-in for the kernels, without a GPU: what they do to tensors, masks and graphs."""
+import pytest
+import torch
+import torch.nn as nn
+from torch.utils.checkpoint import checkpoint
+
+import flashdp4review_b200 as fdp
+from flashdp4review_b200.core import ops
+from flashdp4review_b200.layers import _common
+from oracle import operators as P
+
+
+@pytest.fixture
+def counter(monkeypatch):
+    """A step counter that the stand-in reads as the kernels do: when they run."""
+    c = torch.zeros(1, dtype=torch.int32)
+    monkeypatch.setattr(_common, "_counter_of", lambda x: c)
+
+    def dropout(input, spec, residual=None, out=None):
+        step = spec.step + int(spec.step_device)
+        keep = torch.from_numpy(P.keep_mask(input.numel(), spec.p, spec.seed, spec.stream_id, step, spec.offset)).view(input.shape)
+        y = torch.where(keep, input / (1 - spec.p), 0.0).contiguous()
+        return y if out is None else out.copy_(y)
+
+    monkeypatch.setattr(ops, "dropout", dropout)
+    monkeypatch.setattr(ops, "dropout_backward", lambda g, spec: dropout(g, spec))
+    return c
+
+
+class Two(nn.Module):
+    """a dropout of something that needs no gradient, and one that does"""
+
+    def __init__(self):
+        super().__init__()
+        self.first, self.second = fdp.DPDropout(0.5), fdp.DPDropout(0.5)
+        self.a, self.b = nn.Parameter(torch.ones(1000)), nn.Parameter(torch.ones(1000))
+
+    def forward(self, x):
+        return self.second(self.first(x) * self.a) * self.b
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_recomputed_pass_draws_its_own_step(counter, reentrant):
+    """With the counter on and moved between a checkpoint's passes, the second draws what the first one drew; the gradient of a
+    factor behind the dropouts is the output."""
+    m = Two()
+    x = torch.ones(1000, requires_grad=reentrant)
+    for k in range(3):
+        m.zero_grad()
+        torch.manual_seed(5)                     # (the same seeds in every turn: what is done with is not found again)
+        y = checkpoint(m, x, use_reentrant=reentrant)
+        counter.add_(1)
+        y.sum().backward()
+        assert torch.equal(m.b.grad, y.detach()) and torch.equal(m.a.grad, y.detach()) and 100 < (y != 0).sum() < 400
+    a, b = (checkpoint(m, x, use_reentrant=reentrant) for _ in range(2))       # two graphs at once
+    counter.add_(1)
+    for y in (b, a):
+        m.zero_grad()
+        y.sum().backward(retain_graph=True)
+        assert torch.equal(m.b.grad, y.detach())
+        m.zero_grad()
+        y.sum().backward()                       # (and a graph twice)
+        assert torch.equal(m.b.grad, y.detach())
+    assert not torch.equal(a, b)
+
+
+def test_a_recomputed_pass_that_cannot_be_told_apart_is_refused(counter):
+    m = Two()
+    x = torch.ones(1000)
+    graphs = []
+    for _ in range(2):
+        torch.manual_seed(5)
+        graphs.append(checkpoint(m, x, use_reentrant=False))
+        counter.add_(1)
+    with pytest.raises(RuntimeError, match="same seed"):
+        graphs[0].sum().backward()
+
+
+def test_steps_are_forgotten_with_their_graphs(counter):
+    m = Two()
+    x = torch.ones(1000, requires_grad=True)
+    before = len(_common._drawn)
+    for _ in range(5):
+        m(x).sum().backward()
+    assert len(_common._drawn) == before
+
+
+def test_a_first_pass_that_is_no_longer_known_is_refused(counter, monkeypatch):
+    """Passes without a graph are kept in a bounded number: a checkpoint whose first pass was dropped does not draw another mask."""
+    monkeypatch.setattr(_common, "_GRAPHLESS_MOST", 2)
+    monkeypatch.setattr(_common, "_forgotten", False)
+    _common._graphless.clear()
+    m = Two()
+    x = torch.ones(1000, requires_grad=True)
+    y = checkpoint(m, x, use_reentrant=True)
+    y.sum().backward()                           # (its two dropouts are the two that are kept)
+    y = checkpoint(m, x, use_reentrant=True)
+    with torch.no_grad():
+        for _ in range(3):
+            m.first(x)
+    assert len(_common._graphless) == 2
+    with pytest.raises(RuntimeError, match="no longer known"):
+        y.sum().backward()
