@@ -101,15 +101,19 @@ def dropout_spec(p, stream_id, x, graph=True):
 
     The seed is drawn from torch's CPU generator, which torch.utils.checkpoint restores before it runs a pass again: a count
     of the layer's own would give the recomputed pass another mask than the one whose output the rest of the network has
-    seen.  A data-parallel rank's elements are numbered behind those of the ranks before it, as many as its own: equal
-    shards draw what the whole batch would.  With the device counter on (a step captured in a graph) the step is its value
+    seen.  A data-parallel rank's elements are numbered behind those of the ranks before it, as many groups of eight as its
+    own: equal shards of whole groups draw what the whole batch would.  Shards need not be equal (other lengths, a last batch), so the
+    key holds how many groups the ranks have together if all are like this one: ranks with the same number draw other
+    groups of one stream, ranks with different ones from different streams, whatever their sizes.  With the device counter on (a step captured in a graph) the step is its value
     now, copied on the stream, since it may have moved on by the time the backward runs; a pass that is run again within a backward, by
     its seed, takes the copy of the first one."""
     counter = _counter_of(x)
     if counter is None and x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a captured dropout would draw the same mask on every replay: call use_device_noise_step() first")
-    spec = ops.DropoutSpec(p=p, seed=int(torch.randint(-2 ** 63, 2 ** 63 - 1, (), device="cpu")) & (2 ** 64 - 1), stream_id=stream_id,
-                           offset=runtime.data_parallel()[0] * ((x.numel() + 7) // 8))
+    (rank, world), groups = runtime.data_parallel(), (x.numel() + 7) // 8
+    # (an odd factor: other numbers of groups are other keys)
+    seed = int(torch.randint(-2 ** 63, 2 ** 63 - 1, (), device="cpu")) + groups * world * 0x9E3779B97F4A7C15
+    spec = ops.DropoutSpec(p=p, seed=seed & (2 ** 64 - 1), stream_id=stream_id, offset=rank * groups)
     if counter is not None:
         key = (counter.device, spec.seed, stream_id)
         first = _first_pass(key) if torch._C._current_graph_task_id() != -1 else None

@@ -35,3 +35,17 @@ def test_a_checkpoint_under_a_counter_that_moves(reentrant):
             assert torch.equal(a, b)
     finally:
         fdp.use_device_noise_step(False)
+
+
+def test_unequal_shards_are_dropped_independently():
+    """One seed, shards of ten and six samples: no sample of the second is dropped as one of the first."""
+    m = fdp.DPDropout(0.5)
+    masks = []
+    try:
+        for rank, n in ((0, 10), (1, 6)):
+            fdp.set_data_parallel(rank, 2)
+            torch.manual_seed(7)
+            masks.append(m(torch.ones(n, 64, device=dev())))
+    finally:
+        fdp.set_data_parallel(0, 1)
+    assert not any(torch.equal(a, b) for a in masks[0] for b in masks[1])

@@ -101,3 +101,27 @@ def test_a_first_pass_that_is_no_longer_known_is_refused(counter, monkeypatch):
     assert len(_common._graphless) == 2
     with pytest.raises(RuntimeError, match="no longer known"):
         y.sum().backward()
+
+
+def numbers_of(spec, elements):
+    """which groups of which streams a call draws"""
+    return {(spec.seed, spec.stream_id, spec.offset + g) for g in range((elements + 7) // 8)}
+
+
+@pytest.mark.parametrize("sizes", [(10 * 64, 6 * 64), (6 * 64, 10 * 64), (24, 24, 8), (12, 12), (5, 3), (13, 13, 13), (64, 32, 96, 64), (1, 1)])
+def test_ranks_never_share_a_draw(sizes):
+    """Whatever the sizes of their shards, and with one seed in all of them."""
+    drawn = []
+    try:
+        for rank, n in enumerate(sizes):
+            fdp.set_data_parallel(rank, len(sizes))
+            torch.manual_seed(7)
+            drawn.append(numbers_of(_common.dropout_spec(0.5, 3, torch.empty(n)), n))
+    finally:
+        fdp.set_data_parallel(0, 1)
+    for i, a in enumerate(drawn):
+        for b in drawn[:i]:
+            assert not a & b
+    if len(set(sizes)) == 1 and sizes[0] % 8 == 0:
+        torch.manual_seed(7)
+        assert set().union(*drawn) == numbers_of(_common.dropout_spec(0.5, 3, torch.empty(sum(sizes))), sum(sizes))
