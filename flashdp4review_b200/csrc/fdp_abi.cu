@@ -965,7 +965,7 @@ int fdp_fp8_matmul(const void* x, const void* w, const void* w_packed, const voi
   NvtxRange nvtx_range("fdp_fp8_matmul");
   if (x == nullptr || w == nullptr || w_packed == nullptr || y == nullptr || rows <= 0 || n <= 0 || k <= 0) return FDP_ERR_ARG;
   if (!valid_dtype(dtype) || !valid_dtype(out_dtype)) return FDP_ERR_DTYPE;
-  // (tiles are numbered in 31 bits, with up to 148 parts of a K split)
+  // (tiles are numbered in 31 bits, with up to 16 parts of a K split)
   if (rows > (1 << 30) || n > (1 << 30) || k > (1 << 30) || static_cast<long long>(ceil_div(rows, 128)) * ceil_div(n, 128) >= (1ll << 31) / 256 ||
       static_cast<long long>(ceil_div(rows, 16)) * ceil_div(k, 512) >= (1ll << 31) / 2 || static_cast<long long>(ceil_div(n, 128)) * ceil_div(k, 512) >= (1ll << 31) / 2)
     return FDP_ERR_SHAPE;

@@ -245,10 +245,12 @@ __global__ void __launch_bounds__(256) fp8_weight_kernel(const T* __restrict__ w
 // products wait for is their operands from L2, of which smaller tiles read more: with the quantisation of 16384 rows
 // 1024 -> 4096 78 us against 70, 8192 rows 4096 -> 11008 300 against 284, 8192 rows 2048 -> 2048 55 against 60.)
 //
-// The tensor cores add into their fp32 accumulators by truncation, one unit in the last place a step and all of one sign:
-// with 16-bit outputs that is nothing (344 steps at 11008 columns, 2^-16), with fp32 outputs an accumulator is handed over
-// every F8_CHAIN K blocks and added to registers, rounded to nearest.
-constexpr int F8_BM = 128, F8_THREADS = 320, F8_RING = 160 * 1024, F8_CHAIN = 8;
+// The tensor cores add into their fp32 accumulators by truncation, up to a unit in the last place a step, 2^-23, and all of one
+// sign; a K block has four steps.  So an accumulator is handed over after a number of K blocks and added to registers, rounded to
+// nearest: F8_CHAIN of them for fp32 outputs, and F8_CHAIN_16 for 16-bit ones, whose 512 steps lose at most 2^-14, an eighth to a quarter
+// of fp16's half step (2^-11 to 2^-12).  Contractions of up to 16384 columns have one chain.  (With a single chain of any length 262144
+// columns lost 2^-10.)
+constexpr int F8_BM = 128, F8_THREADS = 320, F8_RING = 160 * 1024, F8_CHAIN = 8, F8_CHAIN_16 = 128;
 template <int CTAS, int BN> struct F8Tile {
   static constexpr int A_BYTES = F8_BM * 128, B_BYTES = BN / CTAS * 128, STG = A_BYTES + B_BYTES;
   static constexpr int STAGES = F8_RING / STG < 8 ? F8_RING / STG : 8;
@@ -641,7 +643,7 @@ int gemm_launch(const Fp8Args& args_in, const void* a, int pitch_a, const void* 
   args.split = pl.split;
   args.m_group = args.tiles_m < 8 ? args.tiles_m : 8;
   args.sticky = sticky_status_slot();
-  args.chain = args.out_dt == FDP_F32 ? F8_CHAIN : args.kblocks;
+  args.chain = args.out_dt == FDP_F32 ? F8_CHAIN : F8_CHAIN_16;
   CUtensorMap ma, mb, msa, msb, mo;
   if (!make_bytes_map(&ma, a, args.M, K, pitch_a, F8_BM) || !make_bytes_map(&mb, w, args.N, K, pitch_w, BN / CTAS) ||
       !make_exponents_map(&msa, sa, args.M, args.kblocks) || !make_exponents_map(&msb, sw, args.N, args.kblocks))

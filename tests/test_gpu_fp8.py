@@ -153,3 +153,27 @@ def test_more_than_2_31_elements(ops, N, K):
     tol = torch.finfo(torch.bfloat16).eps / 2 * few.abs() + 2 * (48 + 8 * -(-K // 128)) * 2.0 ** -24 * mag * 1.01
     assert ((y[-last:].float() - few).abs() <= tol).all()
     assert torch.equal(y[4096 * 254:4096 * 255], y[:4096])      # (of the 256th stretch 164 rows are among the last)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_long_contraction(ops, dtype):
+    """262144 numbers in one accumulator, without a cut along them (144 tiles of 128 x 128).  Numbers that e4m3 holds exactly, so the
+    quantisation loses nothing; the first blocks are much larger than the others, so that what comes after them is cut off.  An accumulator runs
+    for 128 blocks at most, 512 instructions each off by a unit in the last place, 2^-23: with 16-bit outputs too the sum is off by less
+    than 2^-14 of the magnitudes for that (and 48 roundings of the rest; 2^-24 for each of the 16 sums after), then by half a step."""
+    M = N = 1536
+    K = 1 << 18
+    gen = torch.Generator(device=dev()).manual_seed(7)
+    some = lambda r: (torch.randint(8, 16, (r, K), device=dev(), generator=gen) / 8.0).to(dtype)
+    x, w = some(M), some(N)
+    x[:, :128] *= 2.0 ** 12
+    x *= 2.0 ** -8
+    w *= 2.0 ** -8
+    y = ops.fp8_linear_forward(x, ops.fp8_quantize_weight(w))
+    want = x[:64].double() @ w.double().t()
+    assert torch.isfinite(y).all()
+    tol = torch.finfo(dtype).eps / 2 * want + (2.0 ** -14 + 64 * 2.0 ** -24) * want
+    err = (y[:64].double() - want).abs()
+    assert (err <= tol).all(), (err / tol).max()
+    # roundings to the output's type go both ways; what is cut off goes one: the mean of 98304 relative errors shows it alone
+    assert ((y[:64].double() - want) / want).mean().abs() <= 2.0 ** -14
