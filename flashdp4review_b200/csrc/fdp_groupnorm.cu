@@ -399,7 +399,8 @@ template <int V> __device__ __forceinline__ int spread(int c) { return c ^ ((c >
 // A thread takes its sums about the first number that it sees of a channel: the squares then lose nothing to a mean that is
 // large against the spread, and a first number far off the others is itself part of the spread (n deviations about it lose
 // n 2^-24 of what they add up to, n the few rows of a thread; about one number for the whole chunk the same loss has all its
-// rows for n).  What the threads have is put together as (count, mean, squared deviations).
+// rows for n).  What the threads have is put together as (count, mean, squared deviations).  Squares that overflow stay infinite, so
+// that the group's rstd is 0.
 template <typename T, int V>
 __device__ __forceinline__ void gn_stats(const Shape& h, const Share& sh, const Place& pl, uint8_t* gn_raw, const T* x, float2* part) {
   using Stream = Rows<T, V, 1>;
@@ -432,7 +433,7 @@ __device__ __forceinline__ void gn_stats(const Shape& h, const Share& sh, const 
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float m = f1[e] * inv;
-      gn_ent[pl.row * C + spread<V>(col * V + e)] = make_float2(m - fp[e], fmaxf(f2[e] - f1[e] * m, 0.f));
+      gn_ent[pl.row * C + spread<V>(col * V + e)] = make_float2(m - fp[e], isinf(f2[e]) ? f2[e] : fmaxf(f2[e] - f1[e] * m, 0.f));
     }
   }
   __syncthreads();
@@ -547,10 +548,10 @@ __device__ __forceinline__ float2 gn_moments(const Shape& h, const float2* p, in
   }
   return make_float2(ref + off, lanes_sum(m2, lanes));
 }
-// 1 / sqrt(v), one Newton step behind the approximate instruction
+// 1 / sqrt(v), one Newton step behind the approximate instruction; infinite for 0 and 0 for infinity
 __device__ __forceinline__ float inv_sqrt(float v) {
   const float r = rsqrtf(v);
-  return isinf(r) ? r : r * fmaf(-0.5f * v * r, r, 1.5f);
+  return isinf(r) || isinf(v) ? r : r * fmaf(-0.5f * v * r, r, 1.5f);
 }
 __device__ __forceinline__ float2 gn_total(const float2* p, int stride, int chunks, int lanes, int k) {
   float a = 0.f, b = 0.f;

@@ -254,3 +254,23 @@ def test_more_than_2_31_elements(ops):
     for g, name, more in ((res[1], "dgamma", (gerr * xhat.abs() + back["gz"].abs() * xerr).sum(1)), (res[2], "dbeta", gerr.sum(1))):
         per, mag = back[name]
         close(g, N * per.mean(0), torch.zeros(C), torch.float32, N * (lost * mag + more).mean(0))
+
+
+def test_a_variance_beyond_fp32(ops):
+    """Finite numbers whose squared deviations overflow: rstd is 0 and the output the bias, as torch's; the other groups and samples
+    are as they would be."""
+    gen = torch.Generator().manual_seed(12)
+    for B, T, C in ((3, 40, 64), (6, 400, 512)):              # both passes in one kernel; a kernel a pass
+        x = torch.randn(B, T, C, generator=gen)
+        gamma, beta = torch.rand(C, generator=gen) + 0.5, torch.randn(C, generator=gen)
+        y0, st0 = ops.group_norm_forward(x.to(dev()), gamma.to(dev()), beta.to(dev()), 8)
+        x[1, :, :C // 8] *= 1e25
+        x[0, 3, C // 8] = 1e30                              # (one such number is enough)
+        y, st = ops.group_norm_forward(x.to(dev()), gamma.to(dev()), beta.to(dev()), 8)
+        assert (st["rstd"][1, 0] == 0).all() and (st["rstd"][0, 1] == 0).all()
+        cg = C // 8
+        assert torch.equal(y[1, :, :cg], beta[:cg].to(dev()).expand(T, cg)) and torch.equal(y[0, :, cg:2 * cg], beta[cg:2 * cg].to(dev()).expand(T, cg))
+        assert torch.equal(y[2], y0[2]) and torch.equal(y[1, :, cg:], y0[1, :, cg:]) and torch.equal(y[0, :, :cg], y0[0, :, :cg])
+        assert torch.equal(y[0, :, 2 * cg:], y0[0, :, 2 * cg:])
+        dx, dg, db = ops.dp_group_norm_backward(torch.full_like(y, 1e-2), x.to(dev()), gamma.to(dev()), beta.to(dev()), st["mean"], st["rstd"], 8, 1.0, 1.0)
+        assert (dx[1, :, :cg] == 0).all() and all(torch.isfinite(t).all() for t in (dx, dg, db))
