@@ -12,14 +12,22 @@ from .utils import DPParameter as Parameter
 from ._common import DPLayerMixin, dp_scalars, dropout_spec, leaves_a_graph
 
 
+def _channels_first(t):
+    """(B, *, C) as a contiguous (B, C, *) of its own"""
+    t = t.movedim(-1, 1)
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+
+
 class _DPGroupNormFunc(Function):
     @staticmethod
-    def forward(ctx, input, weight, bias, layer, spec):
-        input = input.contiguous()            # (so that the backward does not copy it once more)
-        y, stats = ops.group_norm_forward(input, weight, bias, layer.num_groups, layer.eps, activation=layer.activation, dropout=spec)
-        ctx.save_for_backward(input, weight, bias, stats["mean"], stats["rstd"])
-        ctx.layer, ctx.spec, ctx.activation = layer, spec, layer.activation
-        return y
+    def forward(ctx, input, weight, bias, layer, spec, channels_first):
+        """`channels_first`: input, output and the input's gradient are contiguous (B, C, *)."""
+        x = input.movedim(1, -1) if channels_first else input
+        x = x.contiguous()                    # (so that the backward does not copy it once more)
+        y, stats = ops.group_norm_forward(x, weight, bias, layer.num_groups, layer.eps, activation=layer.activation, dropout=spec)
+        ctx.save_for_backward(x, weight, bias, stats["mean"], stats["rstd"])
+        ctx.layer, ctx.spec, ctx.activation, ctx.channels_first = layer, spec, layer.activation, channels_first
+        return _channels_first(y) if channels_first else y
 
     @staticmethod
     @once_differentiable
@@ -30,18 +38,23 @@ class _DPGroupNormFunc(Function):
         div, noise = dp_scalars(B, layer.noise_multiplier, layer._dp_param_ids[0], layer._next_step(),
                                 param_id2=layer._dp_param_ids[1])
         need_dw = weight is not None and (ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        if ctx.channels_first:
+            grad_output = grad_output.movedim(1, -1)
         dx, dw, db = ops.dp_group_norm_backward(
             grad_output, input, weight, bias, mean, rstd, layer.num_groups, layer.C, layer.clamp_value,
             activation=ctx.activation, dropout=ctx.spec, batch_divisor=div, noise=noise, need_dx=ctx.needs_input_grad[0],
             need_dw=need_dw)
-        return dx, dw if ctx.needs_input_grad[1] else None, db if ctx.needs_input_grad[2] else None, None, None
+        if ctx.channels_first and dx is not None:
+            dx = _channels_first(dx)
+        return dx, dw if ctx.needs_input_grad[1] else None, db if ctx.needs_input_grad[2] else None, None, None, None
 
 
 class DPGroupNorm(nn.GroupNorm, DPLayerMixin):
     """nn.GroupNorm over (B, C, *), with `activation` (None, "relu", "silu", "gelu" or "gelu_tanh") and `dropout` (the
     probability; in training only) behind it in the same kernels.  They work on channels-last storage: an input in
-    torch.channels_last (or channels_last_3d) is taken as it lies, any other is copied once; the output's storage is channels-last either way.
-    `channels_last=True`: input and output are (B, *, C), as those of the Linear layers."""
+    torch.channels_last (or channels_last_3d) is taken as it lies, and output and input gradient have that format too.  For any other they are
+    contiguous, as nn.GroupNorm's, at the price of a copy of each of the input, the output and their gradients.
+    `channels_last=True`: input and output are (B, *, C), as those of the Linear layers, and nothing is copied."""
 
     def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True, device=None, dtype=None,
                  activation=None, dropout: float = 0.0, channels_last: bool = False, C: float = 1.0, clamp_value: float = 1.0,
@@ -64,8 +77,11 @@ class DPGroupNorm(nn.GroupNorm, DPLayerMixin):
         spec = None
         if self.training and self.dropout > 0.0:
             spec = dropout_spec(self.dropout, self._dp_param_ids[2], x, leaves_a_graph(x, self.weight, self.bias))
-        y = _DPGroupNormFunc.apply(x, self.weight, self.bias, self, spec)
-        return y if self.channels_last else y.movedim(-1, 1)
+        if self.channels_last:
+            return _DPGroupNormFunc.apply(x, self.weight, self.bias, self, spec, False)
+        if x.is_contiguous() and (input.dim() in (4, 5) or input.is_contiguous()):      # (of three axes there is no such format)
+            return _DPGroupNormFunc.apply(x, self.weight, self.bias, self, spec, False).movedim(-1, 1)
+        return _DPGroupNormFunc.apply(input, self.weight, self.bias, self, spec, True)
 
     def extra_repr(self):
         return f"{super().extra_repr()}, activation={self.activation}, dropout={self.dropout}"

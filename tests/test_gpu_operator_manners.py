@@ -2,6 +2,7 @@
 import pytest
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
 import flashdp4review_b200 as fdp
@@ -49,3 +50,47 @@ def test_unequal_shards_are_dropped_independently():
     finally:
         fdp.set_data_parallel(0, 1)
     assert not any(torch.equal(a, b) for a in masks[0] for b in masks[1])
+
+
+@pytest.mark.parametrize("shape", [(4, 32, 5, 6), (4, 32, 15), (4, 32), (2, 32, 3, 4, 5), (4, 32, 1), (4, 32, 1, 1), (1, 32, 5, 6)])
+@pytest.mark.parametrize("fmt", ["contiguous", "channels_last", "transposed", "strided"])
+def test_group_norm_keeps_the_memory_order(shape, fmt):
+    """nn.GroupNorm's: output and input gradient of a contiguous input are contiguous, those of one in a channels-last format are
+    in that format, those of any other contiguous; same numbers."""
+    x = torch.randn(shape, device=dev())
+    axes = len(shape) - 2
+    if fmt == "channels_last":
+        if axes < 2:
+            pytest.skip("no such format")
+        x = x.contiguous(memory_format=torch.channels_last if axes == 2 else torch.channels_last_3d)
+    elif fmt == "transposed":
+        x = x.transpose(0, 1).contiguous().transpose(0, 1)
+    elif fmt == "strided":
+        x = torch.randn(shape[:-1] + (2 * shape[-1],), device=dev())[..., ::2]
+    torch.manual_seed(1)
+    m = fdp.DPGroupNorm(8, 32, activation="silu", C=1e6, noise_multiplier=0.0).to(dev())
+    with torch.no_grad():
+        m.weight.normal_(1.0, 0.2)
+        m.bias.normal_(0.0, 0.2)
+    a, b = (x.detach().requires_grad_() for _ in range(2))
+    # (what is in front of the layer sees the gradient as it leaves it; a leaf would be given strides of its own)
+    seen = []
+    ha, hb = a.view_as(a), b.view_as(b)
+    ha.register_hook(seen.append)
+    y, want = m(ha), F.silu(F.group_norm(hb, 8, m.weight, m.bias))
+    g = torch.randn(shape, device=dev())
+    # 2^8 roundings of fp32 of the largest, generously for both
+    assert (y - want).abs().max() <= 2.0 ** -16 * want.abs().max()
+    gb, = torch.autograd.grad(want, b, g)
+    y.backward(g)
+    assert (a.grad - gb).abs().max() <= 2.0 ** -14 * gb.abs().max()
+    if fmt == "channels_last":
+        form = torch.channels_last if axes == 2 else torch.channels_last_3d
+        assert y.is_contiguous(memory_format=form) and seen[0].is_contiguous(memory_format=form)
+    else:
+        assert y.is_contiguous() and seen[0].is_contiguous()
+        assert y.view(shape[0], -1).shape == (shape[0], y.numel() // shape[0])
+    z = m(x.detach())
+    z += 1.0                                       # and both may be changed in place
+    y = m(a * 1.0)
+    y.mul_(2.0).sum().backward()
