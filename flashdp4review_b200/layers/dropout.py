@@ -22,15 +22,19 @@ class _DropoutFunc(Function):
         # elements are numbered in the order of the input's storage; the gradient is brought into the same one
         ctx.order, ctx.spec = _storage_order(input), spec
         x = input.permute(ctx.order)
-        into = inplace and x.is_contiguous()
-        y = ops.dropout(x, spec, residual=None if residual is None else residual.permute(ctx.order), out=x if into else None)
-        y = y.permute(_inverse(ctx.order))
-        if not inplace:
-            return y
-        if not into:
-            input.copy_(y)
-        ctx.mark_dirty(input)
-        return input
+        if inplace:
+            if x.is_contiguous():
+                ops.dropout(x, spec, out=x)
+            else:
+                input.copy_(ops.dropout(x, spec))           # (its axes are in order)
+            ctx.mark_dirty(input)
+            return input
+        if ctx.order == sorted(ctx.order):
+            return ops.dropout(x, spec, residual=residual)
+        # a tensor of the input's strides, written through a permuted view: a view that the Function returned could not be modified in place
+        y = torch.empty_strided(input.shape, input.stride(), dtype=input.dtype, device=input.device)
+        ops.dropout(x, spec, residual=None if residual is None else residual.permute(ctx.order), out=y.permute(ctx.order))
+        return y
 
     @staticmethod
     @once_differentiable

@@ -94,3 +94,21 @@ def test_group_norm_keeps_the_memory_order(shape, fmt):
     z += 1.0                                       # and both may be changed in place
     y = m(a * 1.0)
     y.mul_(2.0).sum().backward()
+
+
+@pytest.mark.parametrize("fmt", ["contiguous", "channels_last", "transposed"])
+def test_a_dropout_may_be_modified_in_place(fmt):
+    x = torch.randn(4, 6, 5, 7, device=dev())
+    x = x.contiguous(memory_format=torch.channels_last) if fmt == "channels_last" else x.transpose(1, 3) if fmt == "transposed" else x
+    x.requires_grad_()
+    m, r = fdp.DPDropout(0.3), torch.randn_like(x)
+    res = []
+    for inplace in (True, False):
+        torch.manual_seed(2)
+        x.grad = None
+        y = m(x)
+        assert y.stride() == x.stride()
+        y = F.relu(y.add_(r), inplace=True) if inplace else F.relu(y + r)
+        y.square().sum().backward()
+        res.append((y.detach(), x.grad))
+    assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])

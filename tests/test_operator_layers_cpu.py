@@ -2,12 +2,35 @@
 import pytest
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
 import flashdp4review_b200 as fdp
 from flashdp4review_b200.core import ops
 from flashdp4review_b200.layers import _common
 from oracle import operators as P
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """dropout by its formula, with the operator's manner of taking and returning tensors"""
+    def dropout(input, spec, residual=None, out=None):
+        assert residual is None or (residual.shape == input.shape and residual.dtype == input.dtype)
+        assert out is None or (out.shape == input.shape and out.is_contiguous())
+        keep = torch.from_numpy(P.keep_mask(input.numel(), spec.p, spec.seed, spec.stream_id, spec.step, spec.offset)).view(input.shape)
+        y = torch.where(keep, input / (1 - spec.p), 0.0).contiguous()
+        y = y if residual is None else y + residual
+        return y if out is None else out.copy_(y)
+
+    monkeypatch.setattr(ops, "dropout", dropout)
+    monkeypatch.setattr(ops, "dropout_backward", lambda g, spec: dropout(g, spec))
+
+
+def stored(fmt):
+    x = torch.randn(4, 6, 5, 7, generator=torch.Generator().manual_seed(1))
+    if fmt == "channels_last":
+        return x.contiguous(memory_format=torch.channels_last)
+    return x.transpose(1, 3) if fmt == "transposed" else x[:, :, ::2] if fmt == "strided" else x
 
 
 @pytest.fixture
@@ -125,3 +148,27 @@ def test_ranks_never_share_a_draw(sizes):
     if len(set(sizes)) == 1 and sizes[0] % 8 == 0:
         torch.manual_seed(7)
         assert set().union(*drawn) == numbers_of(_common.dropout_spec(0.5, 3, torch.empty(sum(sizes))), sum(sizes))
+
+
+@pytest.mark.parametrize("fmt", ["contiguous", "channels_last", "transposed", "strided"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_an_output_may_be_modified_in_place(on_cpu, fmt, residual):
+    """What nn.Dropout's output takes: sums into it, activations in place; with the gradients of the same thing not in place."""
+    m = fdp.DPDropout(0.4)
+    x, r = stored(fmt).requires_grad_(), torch.randn_like(stored(fmt))
+    args = (r,) if residual else ()
+
+    def run(change):
+        torch.manual_seed(3)
+        x.grad = None
+        y = change(m(x, *args))
+        y.square().sum().backward()
+        return y.detach(), x.grad
+
+    pairs = [(lambda y: y.add_(r), lambda y: y + r), (lambda y: y.relu_(), lambda y: y.relu()), (lambda y: F.silu(y, inplace=True), F.silu)]
+    for inplace, plain in pairs:
+        for a, b in zip(run(inplace), run(plain)):
+            assert torch.equal(a, b)
+    y = m(x, *args)
+    y += 1.0
+    assert not y._is_view() and (fmt == "strided" or y.stride() == x.stride())
