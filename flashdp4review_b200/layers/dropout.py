@@ -53,8 +53,8 @@ def _inverse(order):
 
 
 class DPDropout(nn.Dropout):
-    """`forward(input)` drops as nn.Dropout does; `forward(input, residual)` adds `residual` in the same kernel.  In
-    evaluation mode, and for p = 0, the input (or the sum) comes back.  The mask's seed is drawn from torch's CPU generator:
+    """`forward(input)` drops as nn.Dropout does; `forward(input, residual)` adds `residual`, in the same kernel where it has the
+    input's type and shape and with an ordinary sum where not (a 16-bit branch onto an fp32 residual under autocast).  In evaluation mode, and for p = 0, the input (or the sum) comes back.  The mask's seed is drawn from torch's CPU generator:
     torch.manual_seed repeats a run, and torch.utils.checkpoint, which restores that generator, draws a recomputed pass's
     mask again.  Data-parallel ranks draw for their own shards.  In a captured step use_device_noise_step() has to be on
     (every replay then draws anew), else the call is refused."""
@@ -68,5 +68,8 @@ class DPDropout(nn.Dropout):
             return input if residual is None else input + residual
         if self.inplace and residual is not None:
             raise RuntimeError("dropout in place takes no residual")
+        if residual is not None and not (torch.is_tensor(residual) and residual.shape == input.shape and residual.dtype == input.dtype
+                                         and residual.device == input.device):
+            return self.forward(input) + residual
         return _DropoutFunc.apply(input, residual, dropout_spec(self.p, self._stream_id, input, leaves_a_graph(input, residual)),
                                   self.inplace)

@@ -112,3 +112,19 @@ def test_a_dropout_may_be_modified_in_place(fmt):
         y.square().sum().backward()
         res.append((y.detach(), x.grad))
     assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])
+
+
+def test_a_16_bit_branch_onto_an_fp32_residual():
+    """Under autocast: the branch leaves a product in 16 bits, the residual stream is fp32."""
+    lin, drop = fdp.DPLinear(128, 128, noise_multiplier=0.0).to(dev()), fdp.DPDropout(0.3)
+    x = torch.randn(4, 50, 128, device=dev(), requires_grad=True)
+    for training in (True, False):
+        drop.train(training)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            h = lin(x)
+            torch.manual_seed(3)
+            y = drop(h, x)
+            torch.manual_seed(3)
+            want = drop(h) + x
+        assert y.dtype == torch.float32 and torch.equal(y, want)
+        y.sum().backward()

@@ -172,3 +172,19 @@ def test_an_output_may_be_modified_in_place(on_cpu, fmt, residual):
     y = m(x, *args)
     y += 1.0
     assert not y._is_view() and (fmt == "strided" or y.stride() == x.stride())
+
+
+@pytest.mark.parametrize("training", [True, False])
+@pytest.mark.parametrize("case", ["dtype", "shape", "number"])
+def test_a_residual_of_another_type_or_shape(on_cpu, training, case):
+    """The sum that evaluation gives, in training behind the dropout."""
+    m = fdp.DPDropout(0.3).train(training)
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(4, 6, generator=gen).to(torch.bfloat16 if case == "dtype" else torch.float32).requires_grad_()
+    r = torch.randn({"dtype": (4, 6), "shape": (6,), "number": ()}[case], generator=gen).requires_grad_()
+    torch.manual_seed(1)
+    y = m(x, r)
+    torch.manual_seed(1)
+    assert torch.equal(y, m(x) + r) and y.dtype == torch.float32 and y.shape == (4, 6)
+    y.sum().backward()
+    assert x.grad.dtype == x.dtype and torch.equal(r.grad, torch.full(r.shape, 24.0 / max(1, r.numel())))
