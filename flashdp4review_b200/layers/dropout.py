@@ -16,6 +16,18 @@ def _storage_order(x):
     return order if x.permute(order).is_contiguous() else list(range(x.dim()))
 
 
+class _InPlace(Function):
+    """Autograd's own check that `input` may be modified, which it makes behind a Function's forward: here before anything is."""
+    @staticmethod
+    def forward(ctx, input):
+        ctx.mark_dirty(input)
+        return input
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        return grad_output
+
+
 class _DropoutFunc(Function):
     @staticmethod
     def forward(ctx, input, residual, spec, inplace):
@@ -71,5 +83,8 @@ class DPDropout(nn.Dropout):
         if residual is not None and not (torch.is_tensor(residual) and residual.shape == input.shape and residual.dtype == input.dtype
                                          and residual.device == input.device):
             return self.forward(input) + residual
-        return _DropoutFunc.apply(input, residual, dropout_spec(self.p, self._stream_id, input, leaves_a_graph(input, residual)),
-                                  self.inplace)
+        graph = leaves_a_graph(input, residual)
+        if self.inplace and graph:
+            input = _InPlace.apply(input)
+        y = _DropoutFunc.apply(input, residual, dropout_spec(self.p, self._stream_id, input, graph), self.inplace)
+        return input if self.inplace and not graph else y         # (a leaf without a graph comes back as itself)

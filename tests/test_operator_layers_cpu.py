@@ -188,3 +188,19 @@ def test_a_residual_of_another_type_or_shape(on_cpu, training, case):
     assert torch.equal(y, m(x) + r) and y.dtype == torch.float32 and y.shape == (4, 6)
     y.sum().backward()
     assert x.grad.dtype == x.dtype and torch.equal(r.grad, torch.full(r.shape, 24.0 / max(1, r.numel())))
+
+
+@pytest.mark.parametrize("view", [False, True])
+def test_a_leaf_is_refused_before_it_is_overwritten(on_cpu, view):
+    """In place on what autograd does not let be modified: an error, and the numbers stay."""
+    m = fdp.DPDropout(0.5, inplace=True)
+    leaf = torch.ones(4, 8, requires_grad=True)
+    with pytest.raises(RuntimeError, match="in-place|inplace"):
+        m(leaf[:2] if view else leaf)
+    assert torch.equal(leaf, torch.ones(4, 8))
+    parts = (torch.ones(4, 8, requires_grad=True) * 1).unbind(0)
+    with pytest.raises(RuntimeError, match="in-place|inplace"):
+        m(parts[0])
+    assert torch.equal(parts[0], torch.ones(8))
+    with torch.no_grad():
+        assert m(leaf) is leaf and (leaf == 0).any()
