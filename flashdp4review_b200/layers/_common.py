@@ -130,6 +130,14 @@ def leaves_a_graph(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def product_in_8_bits(input, weight):
+    """Whether a Linear or Conv1D layer's call runs its products in 8 bits."""
+    if not runtime.fp8_products() or not input.is_cuda or input.dim() == 0 or weight.dim() != 2:
+        return False
+    dtype = autocast_dtype(input, weight) or input.dtype
+    return ops.fp8_product_ok(dtype, input.numel() // max(1, input.shape[-1]), weight.shape[0], weight.shape[1])
+
+
 def direct_grad_target(param):
     """The bucket slice a DP weight gradient may be written into directly, or None.
 
@@ -168,10 +176,10 @@ _native = None
 
 def native_nodes(input):
     """The call layer with the layers' autograd nodes, or None where the Function classes take the call: tensors that
-    are not on a GPU, products in 8 bits, and torch.jit.trace, which records a Function but would take a node's output
-    for a constant."""
+    are not on a GPU and torch.jit.trace, which records a Function but would take a node's output for a constant.
+    (Products in 8 bits are the Function classes' too: see product_in_8_bits.)"""
     global _native
-    if not input.is_cuda or runtime.fp8_products() or torch._C._get_tracing_state() is not None:
+    if not input.is_cuda or torch._C._get_tracing_state() is not None:
         return None
     if _native is None:
         host = _lib.host()

@@ -15,7 +15,7 @@ from ..core import ops
 from ..core.ops import RuntimeAutoTuner
 from .utils import DPParameter as Parameter
 from ._common import (DPLayerMixin, reshape_to_3d, dp_scalars, autocast_dtype, direct_grad_target,
-                      direct_grad_done, native_nodes, node_state)
+                      direct_grad_done, native_nodes, node_state, product_in_8_bits)
 
 
 class _DPLinearFunc(Function):
@@ -28,7 +28,7 @@ class _DPLinearFunc(Function):
         ctx.layer = layer
         ctx.input_dtype = input.dtype
         ctx.fp8 = None
-        if x.is_cuda and ops.fp8_product_ok(x.dtype, x.numel() // x.shape[-1], w.shape[1], w.shape[0]):
+        if product_in_8_bits(input, weight):
             ctx.fp8 = ops.fp8_quantize_weight(weight, "out_in")     # for the input gradient too
             return ops.fp8_linear_forward(x, ctx.fp8, bias)
         if x.is_cuda and ops.library_product_ok(
@@ -98,7 +98,7 @@ class DPLinear(nn.Linear, DPLayerMixin):
             self.bias = Parameter(self.bias.data)
 
     def forward(self, input):
-        native = native_nodes(input)
+        native = None if product_in_8_bits(input, self.weight) else native_nodes(input)
         if native is not None:
             return native.dp_linear(input, self.weight, self.bias, node_state(self), False, ops.fp32_product_flags())
         return _DPLinearFunc.apply(input, self.weight, self.bias, self)

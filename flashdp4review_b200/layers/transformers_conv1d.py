@@ -32,7 +32,7 @@ from ..core import ops
 from ..core.ops import RuntimeAutoTuner
 from .utils import DPParameter as Parameter
 from ._common import (DPLayerMixin, reshape_to_3d, dp_scalars, autocast_dtype, direct_grad_target,
-                      direct_grad_done, native_nodes, node_state)
+                      direct_grad_done, native_nodes, node_state, product_in_8_bits)
 
 
 class _DPConv1DFunc(Function):
@@ -45,7 +45,7 @@ class _DPConv1DFunc(Function):
         ctx.layer = layer
         ctx.input_dtype = input.dtype
         ctx.fp8 = None
-        if x.is_cuda and ops.fp8_product_ok(x.dtype, x.numel() // x.shape[-1], w.shape[0], w.shape[1]):
+        if product_in_8_bits(input, weight):
             ctx.fp8 = ops.fp8_quantize_weight(weight, "in_out")     # for the input gradient too
             return ops.fp8_linear_forward(x, ctx.fp8, bias)
         if x.is_cuda and ops.library_product_ok(
@@ -120,7 +120,7 @@ class DPConv1D(Conv1D, DPLayerMixin):
 
     def forward(self, x):
         size_out = x.size()[:-1] + (self.nf,)
-        native = None if self.compat_inplace_bias_scale else native_nodes(x)
+        native = None if self.compat_inplace_bias_scale or product_in_8_bits(x, self.weight) else native_nodes(x)
         if native is not None:
             return native.dp_linear(x, self.weight, self.bias, node_state(self), True, ops.fp32_product_flags()).view(size_out)
         return _DPConv1DFunc.apply(self.bias, x, self.weight, self).view(size_out)

@@ -128,3 +128,23 @@ def test_a_16_bit_branch_onto_an_fp32_residual():
             want = drop(h) + x
         assert y.dtype == torch.float32 and torch.equal(y, want)
         y.sum().backward()
+
+
+@pytest.fixture
+def fp8():
+    fdp.set_fp8_products(True)
+    yield
+    fdp.set_fp8_products(False)
+
+
+def test_layers_beside_the_8_bit_products_keep_their_nodes(fp8):
+    """The switch sends a layer to the Function class only for a call that runs in 8 bits."""
+    few, many = torch.randn(2, 20, 192, device=dev(), requires_grad=True), torch.randn(2, 100, 192, device=dev(), requires_grad=True)
+    lin, conv, ln = fdp.DPLinear(192, 256).to(dev()), fdp.DPConv1D(256, 192).to(dev()), fdp.DPLayerNorm(192).to(dev())
+    fdp.set_fp8_products(False)
+    native = [type(m(few).grad_fn).__name__ for m in (lin, ln)] + [type(conv(few).grad_fn.next_functions[0][0]).__name__]
+    fdp.set_fp8_products(True)
+    now = [type(m(few).grad_fn).__name__ for m in (lin, ln)] + [type(conv(few).grad_fn.next_functions[0][0]).__name__]
+    assert now == native and not any("Func" in n and "Backward" in n and n.startswith("_DP") for n in now)
+    assert type(ln(many).grad_fn).__name__ == native[1]
+    assert type(lin(many).grad_fn).__name__ == "_DPLinearFuncBackward"
