@@ -132,10 +132,12 @@ def leaves_a_graph(*tensors):
 
 def product_in_8_bits(input, weight):
     """Whether a Linear or Conv1D layer's call runs its products in 8 bits."""
-    if not runtime.fp8_products() or not input.is_cuda or input.dim() == 0 or weight.dim() != 2:
+    if not runtime.fp8_products() or not input.is_cuda or input.dim() == 0 or input.shape[-1] == 0:
         return False
-    dtype = autocast_dtype(input, weight) or input.dtype
-    return ops.fp8_product_ok(dtype, input.numel() // max(1, input.shape[-1]), weight.shape[0], weight.shape[1])
+    cast, K = autocast_dtype(input, weight), input.shape[-1]
+    dtype, rows, N = cast or input.dtype, input.numel() // K, weight.numel() // K
+    # (a weight of another type than the input's: where the layer takes one without 8 bits too)
+    return ops.fp8_product_ok(dtype, rows, K, N) and (cast is not None or weight.dtype == dtype or ops.library_product_ok(dtype, rows, K, N))
 
 
 def direct_grad_target(param):

@@ -148,3 +148,22 @@ def test_layers_beside_the_8_bit_products_keep_their_nodes(fp8):
     assert now == native and not any("Func" in n and "Backward" in n and n.startswith("_DP") for n in now)
     assert type(ln(many).grad_fn).__name__ == native[1]
     assert type(lin(many).grad_fn).__name__ == "_DPLinearFuncBackward"
+
+
+@pytest.mark.parametrize("shape", [(64, 64), (192, 256), (63, 256), (100, 100)])
+def test_mixed_types_are_answered_or_refused_as_without_8_bits(shape):
+    """A 16-bit input of a layer with fp32 weights, outside autocast."""
+    m = fdp.DPLinear(shape[0], shape[1], noise_multiplier=0.0).to(dev())
+    c = fdp.DPConv1D(shape[1], shape[0], noise_multiplier=0.0).to(dev())
+    x = torch.randn(200, shape[0], device=dev(), dtype=torch.bfloat16)
+    for layer in (m, c):
+        answers = []
+        for on in (False, True):
+            fdp.set_fp8_products(on)
+            try:
+                answers.append(layer(x).dtype)
+            except RuntimeError as e:
+                answers.append("refused")
+            finally:
+                fdp.set_fp8_products(False)
+        assert answers[0] == answers[1]
