@@ -595,15 +595,28 @@ def fp8_quantize_weight(weight, layout="out_in"):
 
 def _fp8_product(x, weight, bias, transposed, out_dtype):
     host = _lib.host()
-    _require_cuda(x, weight.values, bias)
+    w, packed = (weight.values_t, weight.packed_t) if transposed else (weight.values, weight.packed)
+    _require_cuda(x, w, bias)
     code = _dt(x.dtype)
     if x.numel() == 0:
         raise RuntimeError(f"product with an empty operand {tuple(x.shape)}")
-    w, packed = (weight.values_t, weight.packed_t) if transposed else (weight.values, weight.packed)
     b = None if bias is None else bias.to(x.dtype).contiguous()
     st, y = host.fp8_matmul(x.contiguous(), w, packed, b, code, _dt(out_dtype or x.dtype))
     _lib.check(st, "fdp_fp8_matmul")
     return y
+
+
+def fp8_input_grad_tensors(weight):
+    """What `fp8_linear_input_grad` reads of an Fp8Weight, as plain contiguous tensors for an autograd node to save (rows of 8-bit
+    numbers with the padding that belongs to them), and `fp8_input_grad_weight`'s way back."""
+    w, packed = (weight.values_t, weight.packed_t) if weight.layout == "out_in" else (weight.values, weight.packed)
+    return w.as_strided((w.shape[0], w.stride(0)), (w.stride(0), 1)), packed
+
+
+def fp8_input_grad_weight(rows, packed, columns, layout):
+    """An Fp8Weight that is good for the input gradient only, from `fp8_input_grad_tensors` and the columns without padding."""
+    w = rows[:, :columns]
+    return Fp8Weight(None, w, None, None, packed, layout) if layout == "out_in" else Fp8Weight(w, None, None, packed, None, layout)
 
 
 def fp8_linear_forward(input, weight, bias=None, out_dtype=None):

@@ -41,13 +41,15 @@ class _DPConv1DFunc(Function):
         dt = autocast_dtype(input, weight)
         x = input if dt is None else input.to(dt)
         w = weight if dt is None else weight.to(dt)
-        ctx.save_for_backward(bias, x, weight, w if dt is not None else None)
+        saved = (bias, x, weight, w if dt is not None else None)
         ctx.layer = layer
         ctx.input_dtype = input.dtype
-        ctx.fp8 = None
-        if product_in_8_bits(input, weight):
-            ctx.fp8 = ops.fp8_quantize_weight(weight, "in_out")     # for the input gradient too
-            return ops.fp8_linear_forward(x, ctx.fp8, bias)
+        ctx.eight_bits = product_in_8_bits(input, weight)
+        if ctx.eight_bits:
+            w8 = ops.fp8_quantize_weight(weight, "in_out")     # for the input gradient too
+            ctx.save_for_backward(*saved, *(ops.fp8_input_grad_tensors(w8) if ctx.needs_input_grad[1] else ()))
+            return ops.fp8_linear_forward(x, w8, bias)
+        ctx.save_for_backward(*saved)
         if x.is_cuda and ops.library_product_ok(
                 x.dtype, x.numel() // x.shape[-1], w.shape[0], w.shape[1]):
             return ops.linear_forward(x, w, bias, "in_out")     # library GEMM, bias added in its epilogue
@@ -55,7 +57,7 @@ class _DPConv1DFunc(Function):
 
     @staticmethod
     def backward(ctx, grad_output):
-        bias, input, weight, w_cast = ctx.saved_tensors
+        bias, input, weight, w_cast, *w8 = ctx.saved_tensors
         layer = ctx.layer
         w_for_dx = weight if w_cast is None else w_cast
         x3, g3 = reshape_to_3d(input, grad_output)
@@ -73,11 +75,11 @@ class _DPConv1DFunc(Function):
                 grad_bias = None
             need_db = False
 
-        eight_bits = need_dx and ctx.fp8 is not None
+        eight_bits = need_dx and ctx.eight_bits
         native_dx = need_dx and not eight_bits and ops.library_product_ok(
             g3.dtype, g3.numel() // g3.shape[-1], w_for_dx.shape[1], w_for_dx.shape[0])
         if eight_bits:
-            grad_input = ops.fp8_linear_input_grad(g3, ctx.fp8, out_dtype=ctx.input_dtype)
+            grad_input = ops.fp8_linear_input_grad(g3, ops.fp8_input_grad_weight(*w8, weight.shape[1], "in_out"), out_dtype=ctx.input_dtype)
         elif need_dx and not native_dx:
             grad_input = g3 @ w_for_dx.to(g3.dtype).t()
 

@@ -167,3 +167,43 @@ def test_mixed_types_are_answered_or_refused_as_without_8_bits(shape):
             finally:
                 fdp.set_fp8_products(False)
         assert answers[0] == answers[1]
+
+
+@pytest.mark.parametrize("kind", ["linear", "conv1d"])
+@pytest.mark.parametrize("n_in,n_out", [(192, 256), (199, 250)])
+def test_the_8_bit_weight_is_a_saved_tensor(fp8, kind, n_in, n_out):
+    """Seen and moved by saved-tensor hooks (here to the host and back), let go of by the backward, and kept only where an input
+    gradient will ask for it."""
+    m = (fdp.DPLinear(n_in, n_out, noise_multiplier=0.0) if kind == "linear" else fdp.DPConv1D(n_out, n_in, noise_multiplier=0.0)).to(dev())
+    x = torch.randn(2, 100, n_in, device=dev(), requires_grad=True)
+    g = torch.randn(2, 100, n_out, device=dev())
+    m(x).backward(g)
+    want, x.grad = x.grad, None
+    packed = []
+
+    def pack(t):
+        packed.append(t.dtype)
+        return t.cpu()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to(dev())):
+        y = m(x)
+    assert packed.count(torch.float8_e4m3fn) == 1
+    y.backward(g)
+    assert torch.equal(x.grad, want)
+    packed.clear()
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to(dev())):
+        m(x.detach())
+    assert torch.float8_e4m3fn not in packed
+
+
+def test_the_8_bit_weight_does_not_outlive_its_backward(fp8):
+    m = fdp.DPLinear(4096, 4096, noise_multiplier=0.0).to(dev())
+    x = torch.randn(256, 4096, device=dev(), requires_grad=True)
+    torch.autograd.grad(m(x).sum(), [x])                  # (what the library allocates once)
+    torch.cuda.synchronize()
+    start = torch.cuda.memory_allocated()
+    y = m(x)
+    loss = y.sum()
+    dx, = torch.autograd.grad(loss, [x])
+    held = torch.cuda.memory_allocated() - start
+    assert held < y.numel() * 4 + dx.numel() * 4 + (1 << 20)          # output and gradient, not the 16 MB of a weight in 8 bits
