@@ -904,7 +904,8 @@ int fdp_group_norm_bwd(const void* dy, const void* x, const void* gamma, const v
                        size_t workspace_bytes, fdp_stream_t stream) {
   NvtxRange nvtx_range("fdp_group_norm_bwd");
   if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || (gamma == nullptr) != (beta == nullptr) ||
-      (dx == nullptr && dgamma == nullptr) || (dgamma == nullptr) != (dbeta == nullptr) || (dgamma != nullptr && gamma == nullptr))
+      (dx == nullptr && dgamma == nullptr) || (dgamma == nullptr) != (dbeta == nullptr) || (dgamma != nullptr && gamma == nullptr) ||
+      (dgamma == nullptr && (norms_gamma != nullptr || norms_beta != nullptr)))
     return FDP_ERR_ARG;
   int st = check_group_norm(B, T, C, G, activation, dtype, param_dtype, drop);
   if (st != FDP_OK) return st;

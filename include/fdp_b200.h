@@ -336,7 +336,7 @@ int fdp_dropout(const void* x, const void* residual, void* y, size_t n, int dtyp
  *   of y).
  * fdp_group_norm_bwd: dx as autograd's; dgamma / dbeta [C] in `param_dtype` are the per-sample gradients, each clipped by its
  *   norm, summed over the batch / batch_divisor, plus noise (param_id, param_id2), as in fdp_layernorm_bwd.  dx, the pair
- *   dgamma / dbeta and the norms (float[B]) may be NULL; beta is read where there is an activation.
+ *   dgamma / dbeta and the norms (float[B]) may be NULL; norms without the pair are refused; beta is read where there is an activation.
  */
 enum fdp_activation { FDP_ACT_NONE = 0, FDP_ACT_RELU = 1, FDP_ACT_SILU = 2, FDP_ACT_GELU = 3, FDP_ACT_GELU_TANH = 4 };
 size_t fdp_group_norm_fwd_workspace_bytes(int B, int T, int C, int G);

@@ -1,4 +1,6 @@
 """The layers of the operators around a stand-in for the kernels, without a GPU: what they do to tensors, masks and graphs."""
+import ctypes
+
 import pytest
 import torch
 import torch.nn as nn
@@ -6,6 +8,7 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
 import flashdp4review_b200 as fdp
+from flashdp4review_b200 import _lib
 from flashdp4review_b200.core import ops
 from flashdp4review_b200.layers import _common
 from oracle import operators as P
@@ -204,3 +207,12 @@ def test_a_leaf_is_refused_before_it_is_overwritten(on_cpu, view):
     assert torch.equal(parts[0], torch.ones(8))
     with torch.no_grad():
         assert m(leaf) is leaf and (leaf == 0).any()
+
+
+def test_group_norm_norms_come_with_their_gradients():
+    """The norms are by-products of the clipped gradients: a call that asks for norms alone is refused, not left unanswered."""
+    lib, at = _lib.load(), 8192              # (not looked at by a call that is refused)
+    p = _lib.DPParams(1.0, 1.0, 0.0, 0, 1, 1, 2, 1, 0, 1, None)
+    for ng, nb in ((at, at), (at, None), (None, at)):
+        assert lib.fdp_group_norm_bwd(at, at, at, at, at, at, at, None, None, ng, nb, 2, 4, 16, 4, 0, 0, 0, None, ctypes.byref(p), at, 1 << 40,
+                                      None) == _lib.FDP_ERR_ARG
