@@ -73,7 +73,7 @@ class DPDropout(nn.Dropout):
 
     def __init__(self, p: float = 0.5, inplace: bool = False):
         super().__init__(p, inplace)
-        self._stream_id = runtime.next_param_id()
+        self._stream_id = runtime.next_dropout_id()
 
     def forward(self, input, residual=None):
         if not self.training or self.p == 0.0:

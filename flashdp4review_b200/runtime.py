@@ -10,6 +10,7 @@ import itertools
 import os
 
 _ids = itertools.count(1)
+_dropout_ids = itertools.count(1)
 
 
 class _Run:
@@ -244,3 +245,9 @@ def fp8_products():
 def next_param_id() -> int:
     """A fresh id per DP parameter tensor, in construction order."""
     return next(_ids)
+
+
+def next_dropout_id() -> int:
+    """A fresh id per dropout layer.  Not one of the parameters': their noise is a function of their ids, which dropouts between
+    them must not move."""
+    return next(_dropout_ids)

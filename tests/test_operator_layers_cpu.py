@@ -8,7 +8,7 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
 import flashdp4review_b200 as fdp
-from flashdp4review_b200 import _lib
+from flashdp4review_b200 import _lib, runtime
 from flashdp4review_b200.core import ops
 from flashdp4review_b200.layers import _common
 from oracle import operators as P
@@ -216,3 +216,10 @@ def test_group_norm_norms_come_with_their_gradients():
     for ng, nb in ((at, at), (at, None), (None, at)):
         assert lib.fdp_group_norm_bwd(at, at, at, at, at, at, at, None, None, ng, nb, 2, 4, 16, 4, 0, 0, 0, None, ctypes.byref(p), at, 1 << 40,
                                       None) == _lib.FDP_ERR_ARG
+
+
+def test_a_dropout_takes_no_parameter_id():
+    """The noise of a model's parameters is a function of their ids, in construction order: dropouts in between do not move them."""
+    a = runtime.next_param_id()
+    drops = [fdp.DPDropout(0.5) for _ in range(3)]
+    assert runtime.next_param_id() == a + 1 and len({d._stream_id for d in drops}) == 3
