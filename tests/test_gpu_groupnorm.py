@@ -274,3 +274,98 @@ def test_a_variance_beyond_fp32(ops):
         assert torch.equal(y[0, :, 2 * cg:], y0[0, :, 2 * cg:])
         dx, dg, db = ops.dp_group_norm_backward(torch.full_like(y, 1e-2), x.to(dev()), gamma.to(dev()), beta.to(dev()), st["mean"], st["rstd"], 8, 1.0, 1.0)
         assert (dx[1, :, :cg] == 0).all() and all(torch.isfinite(t).all() for t in (dx, dg, db))
+
+
+# ---- tensors that take a kernel a pass -------------------------------------------------------------------------------------
+def launches(call):
+    from flashdp4review_b200 import _lib
+    lib = _lib.load()
+    before = lib.fdp_launch_count()
+    res = call()
+    return lib.fdp_launch_count() - before, res
+
+
+def takes_a_kernel_a_pass(ops, x, w, b, G, act, spec):
+    """(and not clusters: one launch forward, two backward; nor statistics put together by a launch of their own)"""
+    n, (_, st) = launches(lambda: ops.group_norm_forward(x, w, b, G, activation=act, dropout=spec))
+    m, _ = launches(lambda: ops.dp_group_norm_backward(x, x, w, b, st["mean"], st["rstd"], G, 1.0, 1.0, activation=act, dropout=spec))
+    return n == 2 and m == 3
+
+
+# A thread's chain there is of at most 22 rows, a sample has at most 64 chunks, eight of which a thread adds up at most, then eight
+# threads': fewer than the 64 roundings in a row that the tolerances count.
+GRID = [(6, 400, 512, 8, torch.bfloat16), (8, 1600, 90, 6, torch.float16), (8, 1600, 91, 7, torch.bfloat16), (8, 40, 4104, 8, torch.bfloat16),
+        (8, 600, 130, 5, torch.float32), (8, 600, 132, 4, torch.float32), (8, 1600, 90, 90, torch.bfloat16), (8, 40, 4101, 3, torch.float16)]
+
+
+@pytest.mark.parametrize("act,p", [(None, 0.0), ("gelu_tanh", 0.3), ("silu", 0.0)])
+@pytest.mark.parametrize("shape", GRID)
+def test_a_kernel_a_pass(ops, shape, act, p):
+    """Several samples of more than 2 MB together, with whole vectors, rows that are only even, odd rows, and rows of more columns than
+    a block has threads; clipping that bites on some of the samples."""
+    B, T, C, G, dtype = shape
+    spec = ops.DropoutSpec(p=p, seed=11, stream_id=2, step=3) if p else None
+    x, dy, gamma, beta = case(B, T, C, dtype, seed=B + T + C)
+    assert takes_a_kernel_a_pass(ops, x.to(dev()), gamma.to(dev()), beta.to(dev()), G, act, spec)
+    check(ops, x, dy, gamma, beta, G, act, spec)
+
+
+@pytest.mark.parametrize("dropped", [False, True])
+def test_a_kernel_a_pass_on_unaligned_storage(ops, dropped):
+    """What an aligned copy gives, each within its roundings of float64: numbers one by one in place of vectors."""
+    x, dy, gamma, beta = case(6, 400, 512, torch.bfloat16, seed=21)
+    spec = ops.DropoutSpec(p=0.2, seed=5) if dropped else None
+    # a view off 16 bytes stays one through .to() and .contiguous() on its own device
+    off = lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device=dev())[1:].view(t.shape).copy_(t)
+    xo, do = off(x), off(dy)
+    assert xo.data_ptr() % 16 and takes_a_kernel_a_pass(ops, xo, gamma.to(dev()), beta.to(dev()), 8, "silu", spec)
+
+    class Off:
+        """a tensor whose copy on the device is off 16 bytes"""
+        def __init__(self, host, there):
+            self.host, self.there = host, there
+
+        def __getattr__(self, name):
+            return getattr(self.host, name)
+
+        def to(self, *_):
+            return self.there
+
+    check(ops, Off(x, xo), Off(dy, do), gamma, beta, 8, "silu", spec)
+
+
+@pytest.mark.parametrize("shape", [(6, 400, 512, 8), (4, 64, 128, 32)])
+@pytest.mark.parametrize("p", [0.0, 0.3])
+def test_parts_of_a_backward(ops, shape, p):
+    """Without the input's gradient, or without the parameters', the rest has the same bits."""
+    B, T, C, G = shape
+    x, dy, gamma, beta = (t.to(dev()) for t in case(B, T, C, torch.bfloat16, seed=22))
+    spec = ops.DropoutSpec(p=p, seed=5) if p else None
+    _, st = ops.group_norm_forward(x, gamma, beta, G, activation="gelu", dropout=spec)
+    back = lambda **k: ops.dp_group_norm_backward(dy, x, gamma, beta, st["mean"], st["rstd"], G, 0.5, 1.0, activation="gelu", dropout=spec, return_norms=True, **k)
+    whole, no_dx, no_dw = back(), back(need_dx=False), back(need_dw=False)
+    assert no_dx[0] is None and all(torch.equal(a, b) for a, b in zip(whole[1:], no_dx[1:]))
+    assert torch.equal(no_dw[0], whole[0]) and no_dw[1:] == (None,) * 4
+
+
+def test_many_samples_in_a_kernel_a_pass(ops):
+    """More samples than the clipped sum keeps factors of in shared memory, of more than 2 MB together."""
+    B, T, C, G = 9000, 8, 16, 2
+    x, dy, w, b = case(B, T, C, torch.float32, seed=25)
+    y, mean, rstd, xhat, z = P.group_norm(x, w, b, G, 1e-5, None, None, 0.0)
+    n, (_, st) = launches(lambda: ops.group_norm_forward(x.to(dev()), w.to(dev()), b.to(dev()), G))
+    assert n == 2
+    res = ops.dp_group_norm_backward(dy.to(dev()), x.to(dev()), w.to(dev()), b.to(dev()), st["mean"], st["rstd"], G, 0.2, 1.0, return_norms=True)
+    want = P.group_norm_backward(dy, w, rstd, xhat, z, G, None, None, 0.0)
+    xerr = FP32 * ((x.double().abs() + mean.abs().repeat_interleave(C // G, 1)[:, None]) * rstd.repeat_interleave(C // G, 1)[:, None] + 2)
+    for got, norms, name, more in ((res[1], res[3], "dgamma", (dy.double().abs() * xerr).sum(1)), (res[2], res[4], "dbeta", 0.0)):
+        per, mag = want[name]
+        mean_, n_ = P.clipped_mean(per, 0.2, 1.0)
+        assert 0 < (n_ > 0.2).sum() < B
+        err = FP32 * mag + more
+        nerr = err.square().sum(1).sqrt() + FP32 * n_
+        assert ((norms.double().cpu() - n_).abs() <= nerr + 1e-30).all()
+        f = torch.from_numpy(O.clip_factor(n_.numpy(), 0.2, 1.0))
+        # the sum over the samples is a chain of at most B additions, each off by 2^-24 of the magnitudes so far
+        tol = (err * f[:, None] + per.abs() * (f * (nerr / n_.clamp(min=1e-30) + FP32 + B * 2.0 ** -24))[:, None]).sum(0) / B
+        close(got, mean_, torch.zeros_like(mean_), torch.float32, tol)

@@ -207,3 +207,25 @@ def test_the_8_bit_weight_does_not_outlive_its_backward(fp8):
     dx, = torch.autograd.grad(loss, [x])
     held = torch.cuda.memory_allocated() - start
     assert held < y.numel() * 4 + dx.numel() * 4 + (1 << 20)          # output and gradient, not the 16 MB of a weight in 8 bits
+
+
+def test_group_norm_gradients_through_the_reducer():
+    """A group norm's gradients in the buckets of the data-parallel reducer are those without it, accumulated and started anew."""
+    from flashdp4review_b200.distributed import DPGradReducer
+
+    def make():
+        torch.manual_seed(1)
+        return nn.Sequential(fdp.DPGroupNorm(4, 32, activation="silu", channels_last=True, C=0.3, noise_multiplier=0.0),
+                             fdp.DPLinear(32, 50, C=0.3, noise_multiplier=0.0)).to(dev())
+
+    x, g = torch.randn(4, 6, 32, device=dev()), torch.randn(4, 6, 50, device=dev()) * 0.1
+    plain, model = make(), make()
+    plain(x).backward(g)
+    red = DPGradReducer(model, bucket_bytes=1 << 12, grad_as_bucket_view=True)
+    for again in (False, True):
+        model(x).backward(g)
+        red.finish()
+        for p, q in zip(model.parameters(), plain.parameters()):
+            assert p.grad.data_ptr() == red._views[id(p)].data_ptr() and torch.equal(p.grad, q.grad)
+        red.zero_grad()
+    red.remove()
