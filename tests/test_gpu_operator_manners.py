@@ -229,3 +229,41 @@ def test_group_norm_gradients_through_the_reducer():
             assert p.grad.data_ptr() == red._views[id(p)].data_ptr() and torch.equal(p.grad, q.grad)
         red.zero_grad()
     red.remove()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_captured_checkpoint(reentrant):
+    """A checkpointed dropout in a captured step whose counter moves before the backward: in every replay the gradient of a factor behind
+    it is the output, and every replay draws anew."""
+    m = fdp.DPDropout(0.5)
+    fdp.use_device_noise_step(True)
+    try:
+        x, w = (torch.ones(1000, device=dev(), requires_grad=True) for _ in range(2))
+
+        def step():
+            y = checkpoint(lambda t: m(t) * w, x, use_reentrant=reentrant)
+            fdp.advance_noise_step()
+            y.sum().backward()
+            return y.detach()
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        w.grad = x.grad = None
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = step()
+        seen = []
+        for _ in range(2):
+            w.grad.zero_()
+            x.grad.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(w.grad, y) and torch.equal(x.grad, y)
+            seen.append(y.clone())
+        assert not torch.equal(*seen)
+    finally:
+        fdp.use_device_noise_step(False)
