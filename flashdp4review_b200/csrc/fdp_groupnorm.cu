@@ -10,11 +10,12 @@
 // Each direction reads its inputs twice, reductions first, then the result; the second pass runs from the back, so that what
 // the first one read last is still in L2.  A row is C contiguous numbers; a thread keeps one column (16 bytes) of channels
 // and walks rows, so that channel sums and parameters stay in registers.  All sums run in a fixed order.  What bounds it is
-// instruction issue as much as memory: at the memory's speed a 16-bit element leaves 22 issue slots for a read and a write or two
-// reads; the statistics take 10, the other passes 14 to 18 with silu and 25 to 33 with gelu and dropout, a third of that
-// what a block does beside its rows.  16 x 4096 x 320 bf16 with silu: 77 us both ways (the reads and writes of both
+// latency and the ends of passes: 46 to 62 % of the issue slots are used, by 22 to 35 % of the warps that an SM could hold (80
+// registers, with dropout 127), and a pass's start and end move nothing.  (At the memory's speed a 16-bit element leaves 22 issue slots
+// for a read and a write or two reads; the statistics take 10, the other passes 14 to 18 with silu and 25 to 33 with gelu and
+// dropout, a third of that what a block does beside its rows.)  16 x 4096 x 320 bf16 with silu: 77 us both ways (the reads and writes of both
 // ways once: 32); with 16 x 324 x 320 a pass takes 7 to 13 us from cold, so its start and end are much of it.  8 x 16384 x 256
-// fp32, whose tensors do not stay in L2: 191 us of 164.
+// fp32, whose tensors do not stay in L2: 190 us of 164.
 // (Tried: one kernel a direction whose blocks draw reductions and results from a counter, so that nothing drains between the
 // passes.  A block that drew a result waited for reductions still running beside it: 16 x 4096 x 320 bf16 144 us for both
 // directions against 117 then with a kernel a pass.  Tried: sets of samples whose second pass finds all of them in L2:
@@ -1097,7 +1098,8 @@ int bwd_drop(const GnArgs& a, const GnPlan& pl, bool need_dw, int* nparts, cudaS
 // Small tensors, where launches are what counts: clusters.  A sample's groups go to `slabs` clusters, its rows to the `chunks`
 // blocks of each, and both passes are one kernel.  On the device a kernel a pass is as fast or faster (16 x 64 x 256 bf16, forward
 // and backward 5.8 + 8.5 us against 6.9 + 9.8; 2 x 1600 x 256 13.0 + 14.3 against 8.8 + 14.3), but up to 2 MB a call takes the host
-// longer than either, and a launch more is 2 to 3 us of it.  (Rows of a slab are at least 64 bytes, where they are no vectors 32:
+// longer than either, and a launch more is 2 to 3 us of it.  (In a captured step the host's time does not count and the difference on
+// the device is lost.  Rows of a slab are at least 64 bytes, where they are no vectors 32:
 // 3 x 1369 x 90 fp16 backward 13.1 us with one slab, 11.8 with three.)
 // Others: a kernel a pass over whole rows, which keeps the SMs fuller (16 x 4096 x 320 bf16: 91 us then, in clusters of 16 blocks
 // 113 to 142), in the number of chunks that takes the fewest (rows a thread + fixed cost of a block) a wave of blocks.

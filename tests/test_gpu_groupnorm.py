@@ -3,8 +3,8 @@
 Tolerances.  A stored result is off by at most half a step of its type (finfo.eps / 2 of its value).  What comes before that is
 fp32: a result passes through fewer than 64 roundings in a row -- a thread's chain of at most 4 + T / (chunks * rows at a time) additions, the
 chunks' chain, a dozen operations of the formula, and at the sizes here never more -- each at most 2^-24 of the sum of
-the magnitudes that it is made of, which the oracle returns: 2^-18 of that in all.  The fast exponential of 16-bit tensors
-(2^-21 relative) is inside the same 2^-18.  Where a relu's argument is within 2^-16 of zero its slope may come out as
+the magnitudes that it is made of, which the oracle returns: 2^-18 of that in all.  The fast exponential and reciprocal
+(2^-21 relative, for every type) are inside the same 2^-18.  Where a relu's argument is within 2^-16 of zero its slope may come out as
 either of 0 and 1; sums may then miss those terms.
 """
 import math
