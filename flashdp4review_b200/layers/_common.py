@@ -74,8 +74,8 @@ def _remember(key, spec, graph):
         else:
             _drawn.pop(key, None)
 
-    # (under a seed that is used again, what has been run again already is done with)
-    live = [r for r in _drawn.get(key, ()) if r() is not None and not r().run_again]
+    # (under a seed that is used again, what has no graph and has been run again already is done with)
+    live = [r for r in _drawn.get(key, ()) if r() is not None and (r().graph or not r().run_again)]
     _drawn[key] = live + [weakref.ref(spec, gone)]
     if not graph:
         _graphless.append(spec)
@@ -121,7 +121,7 @@ def dropout_spec(p, stream_id, x, graph=True):
             first.run_again = True
             spec.step_device = first.step_device
         else:
-            spec.step_device, spec.run_again = counter.clone(), False
+            spec.step_device, spec.graph, spec.run_again = counter.clone(), graph, False
             _remember(key, spec, graph)
     return spec
 

@@ -223,3 +223,21 @@ def test_a_dropout_takes_no_parameter_id():
     a = runtime.next_param_id()
     drops = [fdp.DPDropout(0.5) for _ in range(3)]
     assert runtime.next_param_id() == a + 1 and len({d._stream_id for d in drops}) == 3
+
+
+def test_a_kept_graph_is_not_taken_for_a_later_one(counter):
+    """Run again once, kept, and run again after another pass under its seed: refused, since the steps differ."""
+    m = Two()
+    x = torch.ones(1000, requires_grad=True)
+    torch.manual_seed(5)
+    y = checkpoint(m, x, use_reentrant=False)
+    y.sum().backward(retain_graph=True)
+    counter.add_(1)
+    torch.manual_seed(5)
+    other = checkpoint(m, x, use_reentrant=False)
+    with pytest.raises(RuntimeError, match="same seed"):
+        y.sum().backward()
+    del other
+    m.zero_grad()
+    y.sum().backward()
+    assert torch.equal(m.b.grad, y.detach())
