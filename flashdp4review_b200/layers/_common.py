@@ -52,8 +52,8 @@ def dp_scalars(local_batch, noise_multiplier, param_id, step, param_id2=0):
 
 
 # The specs of passes that drew at a step of the device counter, by (device, seed, stream): a pass that
-# torch.utils.checkpoint runs again finds the step of the first one there.  A pass's graph keeps its spec; one that leaves no graph (the
-# first pass of a reentrant checkpoint, or a dropout of something that needs no gradient) is kept in `_graphless`.
+# torch.utils.checkpoint runs again finds the step of the first one there.  A pass's graph keeps its spec; one that leaves no
+# graph (the first pass of a reentrant checkpoint, or a dropout of something that needs no gradient) is kept in `_graphless`.
 _drawn = {}
 _graphless = collections.deque()
 _GRAPHLESS_MOST = 1 << 14
@@ -102,11 +102,11 @@ def dropout_spec(p, stream_id, x, graph=True):
     The seed is drawn from torch's CPU generator, which torch.utils.checkpoint restores before it runs a pass again: a count
     of the layer's own would give the recomputed pass another mask than the one whose output the rest of the network has
     seen.  A data-parallel rank's elements are numbered behind those of the ranks before it, as many groups of eight as its
-    own: equal shards of whole groups draw what the whole batch would.  Shards need not be equal (other lengths, a last batch), so the
-    key holds how many groups the ranks have together if all are like this one: ranks with the same number draw other
-    groups of one stream, ranks with different ones from different streams, whatever their sizes.  With the device counter on (a step captured in a graph) the step is its value
-    now, copied on the stream, since it may have moved on by the time the backward runs; a pass that is run again within a backward, by
-    its seed, takes the copy of the first one."""
+    own: equal shards of whole groups draw what the whole batch would.  Shards need not be equal (other lengths, a last batch),
+    so the key holds how many groups the ranks have together if all are like this one: ranks with the same number draw other
+    groups of one stream, ranks with different ones from different streams, whatever their sizes.  With the device counter on
+    (a step captured in a graph) the step is its value now, copied on the stream, since it may have moved on by the time the
+    backward runs; a pass that is run again within a backward is known by its seed and takes the copy of the first one."""
     counter = _counter_of(x)
     if counter is None and x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a captured dropout would draw the same mask on every replay: call use_device_noise_step() first")

@@ -66,11 +66,13 @@ def _inverse(order):
 
 class DPDropout(nn.Dropout):
     """`forward(input)` drops as nn.Dropout does; `forward(input, residual)` adds `residual`, in the same kernel where it has the
-    input's type and shape and with an ordinary sum where not (a 16-bit branch onto an fp32 residual under autocast).  In evaluation mode, and for p = 0, the input (or the sum) comes back.  The mask's seed is drawn from torch's CPU generator:
+    input's type and shape and with an ordinary sum where not (a 16-bit branch onto an fp32 residual under autocast).  In
+    evaluation mode, and for p = 0, the input (or the sum) comes back.  The mask's seed is drawn from torch's CPU generator:
     torch.manual_seed repeats a run, and torch.utils.checkpoint, which restores that generator, draws a recomputed pass's
-    mask again.  With use_device_noise_step() on, such a pass is known by its seed: two graphs that drew from one seed at different steps cannot be
-    told apart, and running one of them again is refused.  Data-parallel ranks draw for their own shards, whatever their sizes.  In a captured step use_device_noise_step() has to be on
-    (every replay then draws anew), else the call is refused."""
+    mask again.  With use_device_noise_step() on, such a pass is known by its seed: two graphs that drew from one seed at
+    different steps cannot be told apart, and running one of them again is refused.  Data-parallel ranks draw for their own
+    shards, whatever their sizes.  In a captured step use_device_noise_step() has to be on (every replay then draws anew), else
+    the call is refused."""
 
     def __init__(self, p: float = 0.5, inplace: bool = False):
         super().__init__(p, inplace)

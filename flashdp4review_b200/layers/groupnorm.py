@@ -52,10 +52,9 @@ class _DPGroupNormFunc(Function):
 class DPGroupNorm(nn.GroupNorm, DPLayerMixin):
     """nn.GroupNorm over (B, C, *), with `activation` (None, "relu", "silu", "gelu" or "gelu_tanh") and `dropout` (the
     probability; in training only) behind it in the same kernels.  They work on channels-last storage: an input in
-    torch.channels_last (or channels_last_3d) is taken as it lies, and output and input gradient have that format too.  For any other they are
-    contiguous, as nn.GroupNorm's, at the price of a copy of each of the input, the output and their gradients.
-    `channels_last=True`: input and output are (B, *, C), as those of the Linear layers, and nothing is copied.
-    (16 x 320 x 64 x 64 bf16 with silu, forward and backward: 106 us in channels_last, 434 contiguous; 8 x 256 x 128 x 128 fp32 190
+    torch.channels_last (or channels_last_3d) is taken as it lies, and output and input gradient have that format too.  For any
+    other they are contiguous, as nn.GroupNorm's, at the price of a copy of each of the input, the output and their gradients.
+    `channels_last=True`: input and output are (B, *, C), as those of the Linear layers, and nothing is copied.  (16 x 320 x 64 x 64 bf16 with silu, forward and backward: 106 us in channels_last, 434 contiguous; 8 x 256 x 128 x 128 fp32 190
     and 760.)  The output has the input's type, under autocast too."""
 
     def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True, device=None, dtype=None,
